@@ -911,6 +911,8 @@ __device__ __forceinline__ float sum_np_order(const float* a, int n) {      // n
 
 __global__ void bank_policy_kernel(int32_t* maps, rmem_bank_state* st, const float* __restrict__ w_raw, int n_att, int cap,
                                    int former, int32_t* result) {
+  // plain operators under this pragma: __fmul_rn / __fadd_rn are ordinary operations to the compiler, which may join them to an fma
+#pragma clang fp contract(off)
   if (threadIdx.x != 0) return;
   const int T = st->T;                               // includes the slot appended by this update (not attended)
   if (n_att > T) n_att = T;
@@ -919,7 +921,7 @@ __global__ void bank_policy_kernel(int32_t* maps, rmem_bank_state* st, const flo
   const float wsum = sum_np_order(w, n_att);
   for (int i = 0; i < n_att; ++i) {                  // normalise, moving mean over the slots seen before (:905-928)
     float x = __fdiv_rn(w[i], wsum);
-    if (st->has_ema[i]) x = __fadd_rn(__fmul_rn(0.2f, st->ema[i]), __fmul_rn(0.8f, x));
+    if (st->has_ema[i]) x = 0.2f * st->ema[i] + 0.8f * x;
     w[i] = x;
     st->ema[i] = x;
     st->has_ema[i] = 1;
@@ -935,7 +937,7 @@ __global__ void bank_policy_kernel(int32_t* maps, rmem_bank_state* st, const flo
     if (n_att > 1) {
       float best = 0.f;
       for (int i = 1; i < n_att; ++i) {
-        const float score = __fadd_rn(w[i], __fmul_rn(1.5f, __fsqrt_rn(__fdiv_rn(lg, __fadd_rn(c[i], 8.0f)))));
+        const float score = w[i] + 1.5f * __fsqrt_rn(__fdiv_rn(lg, c[i] + 8.0f));
         if (i == 1 || score < best) {
           best = score;
           drop = i;
