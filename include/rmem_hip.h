@@ -456,6 +456,101 @@ int rmem_labels_from_logits(const rmem_label_src *srcs, int32_t n_src, int32_t C
 int rmem_label_resize_nearest(const uint8_t *src, int32_t Hs, int32_t Ws, uint8_t *dst,
                               int32_t Hd, int32_t Wd, int32_t flip, void *stream);
 
+/* ------------------------------------------------------------------ paged 8-bit bank
+ * A memory bank for many requests (clips, streams) of unequal length: one pool of pages, one byte per element, one scale per
+ * (page, head) for the keys and one for the values.  The banks above are dense, one clip each, every slot of one geometry; here
+ * a request's tokens lie in the pages that its row of a block table names, so requests grow, end and share one pool without
+ * copies.
+ *
+ *   rmem_bank8_plan    lengths -> block tables, slot map, row offsets; takes pages from and returns them to a ring, on the device
+ *   rmem_bank8_append  new tokens -> codes
+ *   rmem_bank8_gather  tokens by slot -> dense values
+ *   rmem_bank8_attn    attention of each request's rows over its pages
+ *
+ * Element = code * scale.  code 0 ("int8"): integer -127..127, held as the byte code + 128; code 1 ("e4m3"): the bits of the
+ * 8-bit float with 4 exponent and 3 mantissa bits, largest value 448, no infinities.  Scales are positive and finite.
+ *   keys    [pages][heads][dim/16][page][16]
+ *   values  [pages][heads][page/32][2][dim][16]   byte 4 m + r of half h = token 8 m + 4 h + r of the 32-token tile
+ * slot = page_id * page + token in the page.  All pointers 16-byte aligned.  None of these calls is recordable (rmem_rec_*). */
+typedef struct {
+  uint8_t *k, *v;
+  float *k_scale, *v_scale;                /* [pages][heads]                                                  */
+  int32_t pages, heads, page, dim, code;   /* page 32, 64 or 128 tokens; dim 32, 64 or 128; pages * page < 2^31 */
+} rmem_bank8;
+
+/* Block tables and slot map of one step, in one launch (a second one maps slots when there are many rows).  Request r keeps its
+ * first ctx[r] tokens and wants add[r] more (negative lengths count as 0); its rows are rows cu[r] .. cu[r+1] of the step.
+ * In request order, requests are granted their pages while the ring has enough: r is granted if its tokens fit into `cols` pages
+ * and either it needs no new page or the pages asked for by requests 0..r (those that fit their row) are at most the ring's.
+ * A request that is not granted keeps lens = ctx and gets slots -1; it has to be asked for again.
+ * had (or NULL): tokens each request held before; pages table[r][ceil(ctx/page)] .. table[r][ceil(had/page) - 1] go back to the
+ * end of the ring, from where later calls take them (had > ctx: a request that ended or was cut).
+ * free_ring [ring] with state = {head, count}: count free pages from position head on, modulo ring.  state_out may be state_in,
+ * lens may be ctx.  rows >= the sum of add: slots past it are -1. */
+typedef struct {
+  const int32_t *ctx, *add, *had; int32_t reqs;
+  int32_t *table; int64_t ld_table; int32_t cols;   /* [reqs][ld_table], cols used; only new entries are written */
+  int32_t page;
+  int32_t *free_ring; int32_t ring;
+  const int32_t *state_in; int32_t *state_out;      /* {head, count}                                       */
+  int32_t *cu;                                      /* [reqs + 1] first row of each request                */
+  int32_t *lens;                                    /* [reqs] tokens held afterwards                       */
+  int32_t *start;                                   /* [reqs] position of the first new token; -1: not granted */
+  int32_t *slots; int32_t rows;                     /* [rows]                                              */
+  int32_t *status;                                  /* [2] pages taken, pages missing                      */
+} rmem_bank8_plan_args;
+int rmem_bank8_plan(const rmem_bank8_plan_args *a, void *stream);
+
+/* Writes rows of new tokens (type 0 fp32, 1 fp16, 2 bf16; strides in elements, dim contiguous) to slots[row]; a row whose slot
+ * lies outside the pool (-1) is skipped and not read; of several rows with one slot the last counts.  The rows of a call that go
+ * to one page, in whatever order, are written together.  If the page's first place is among theirs the page begins anew: what it
+ * held is gone, places between them are 0.  Otherwise the places in front of and between them are kept.  The rest of the last
+ * 32-token tile of values becomes 0.
+ * Per (page, head): scale = max|x| / top (top 127 or 448; max|x| over the finite values, at least 1e-30), or the page's former
+ * scale where it kept tokens and that is larger; where the scale rises the kept codes are rounded again,
+ * code' = rn(code * (old / new)).  code = rn(x * (1 / scale)), saturating; NaN becomes 0, an infinity the largest code.
+ * workspace: rmem_bank8_append_workspace(a) bytes (0 up to 4096 rows), 16-byte aligned, of this call alone until it has run. */
+typedef struct {
+  rmem_bank8 bank;
+  const void *k, *v; int32_t type;
+  int64_t k_row, k_head, v_row, v_head;             /* strides of row and head */
+  const int32_t *slots; int32_t rows;               /* rows < 2^24 */
+  void *workspace; int64_t workspace_bytes;
+} rmem_bank8_append_args;
+int64_t rmem_bank8_append_workspace(const rmem_bank8_append_args *a);   /* -1: invalid arguments */
+int rmem_bank8_append(const rmem_bank8_append_args *a, void *stream);
+
+/* out[row] = code * scale of slot slots[row], rounded to `type`; zeros where the slot lies outside the pool.
+ * ko, vo: [rows][heads][dim], contiguous, 16-byte aligned. */
+typedef struct {
+  rmem_bank8 bank;
+  const int32_t *slots; int32_t rows;
+  void *ko, *vo; int32_t type;
+} rmem_bank8_gather_args;
+int rmem_bank8_gather(const rmem_bank8_gather_args *a, void *stream);
+
+/* out_i = sum_j softmax_j(scale * q_i . k_j) v_j over the tokens j that row i sees; lse_i = log sum_j exp(scale * q_i . k_j).
+ * Request r's rows are cu[r] .. cu[r+1] (limited to rows), its tokens the first lens[r] of its row of the table (limited to
+ * cols * page).  causal: row i of n sees tokens j <= len - n + i, otherwise all.  A row that sees nothing gets 0 and -inf; rows
+ * past cu[reqs] are left as they were.  A table entry outside the pool stands for a page that nobody sees.
+ * heads_q = a multiple of bank.heads: query head h reads head h / (heads_q / bank.heads).  q, out of `type` with strides in
+ * elements and dim contiguous; lse [rows][heads_q] fp32 or NULL.  scale > 0.  max_rows: the largest number of rows of a request,
+ * as far as known (it selects kernels; any value is safe).  Scores, weights and sums are fp32; q counts with 22 bits, values of
+ * fp32 calls with 22-bit weights, of 16-bit calls with 11-bit weights.  Value scales below 2^-96 are read as 2^-96.
+ * workspace: rmem_bank8_attn_workspace(a) bytes, 16-byte aligned, of this call alone until it has run. */
+typedef struct {
+  rmem_bank8 bank;
+  const void *q; void *out; float *lse; int32_t type;
+  int64_t q_row, q_head, o_row, o_head;
+  const int32_t *cu, *lens; int32_t reqs, rows;
+  const int32_t *table; int64_t ld_table; int32_t cols;
+  int32_t heads_q, max_rows, causal;
+  float scale;
+  void *workspace; int64_t workspace_bytes;
+} rmem_bank8_attn_args;
+int64_t rmem_bank8_attn_workspace(const rmem_bank8_attn_args *a);   /* -1: invalid arguments */
+int rmem_bank8_attn(const rmem_bank8_attn_args *a, void *stream);
+
 /* ---- several clips' memory banks in one launch -------------------------------
  * The reference serves one clip per call: its attention asserts batch 1
  * (aot_plus/networks/layers/transformer.py:641,1190) and the evaluator walks clips one after the

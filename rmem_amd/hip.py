@@ -105,6 +105,43 @@ class LabelSrc(C.Structure):
     _fields_ = [("logits", c_p), ("h", i32), ("w", i32), ("flip", i32)]
 
 
+class Bank8Args(C.Structure):
+    _fields_ = [("k", c_p), ("v", c_p), ("k_scale", c_p), ("v_scale", c_p),
+                ("pages", i32), ("heads", i32), ("page", i32), ("dim", i32), ("code", i32)]
+
+
+class Bank8PlanArgs(C.Structure):
+    _fields_ = [
+        ("ctx", c_p), ("add", c_p), ("had", c_p), ("reqs", i32),
+        ("table", c_p), ("ld_table", i64), ("cols", i32), ("page", i32),
+        ("free_ring", c_p), ("ring", i32), ("state_in", c_p), ("state_out", c_p),
+        ("cu", c_p), ("lens", c_p), ("start", c_p), ("slots", c_p), ("rows", i32), ("status", c_p),
+    ]
+
+
+class Bank8AppendArgs(C.Structure):
+    _fields_ = [
+        ("bank", Bank8Args), ("k", c_p), ("v", c_p), ("type", i32),
+        ("k_row", i64), ("k_head", i64), ("v_row", i64), ("v_head", i64), ("slots", c_p), ("rows", i32),
+        ("workspace", c_p), ("workspace_bytes", i64),
+    ]
+
+
+class Bank8GatherArgs(C.Structure):
+    _fields_ = [("bank", Bank8Args), ("slots", c_p), ("rows", i32), ("ko", c_p), ("vo", c_p), ("type", i32)]
+
+
+class Bank8AttnArgs(C.Structure):
+    _fields_ = [
+        ("bank", Bank8Args), ("q", c_p), ("out", c_p), ("lse", c_p), ("type", i32),
+        ("q_row", i64), ("q_head", i64), ("o_row", i64), ("o_head", i64),
+        ("cu", c_p), ("lens", c_p), ("reqs", i32), ("rows", i32),
+        ("table", c_p), ("ld_table", i64), ("cols", i32),
+        ("heads_q", i32), ("max_rows", i32), ("causal", i32), ("scale", f32),
+        ("workspace", c_p), ("workspace_bytes", i64),
+    ]
+
+
 EXPORTS = [
     "rmem_abi_version", "rmem_configure", "rmem_set_host_wait", "rmem_linear", "rmem_linear_trace",
     "rmem_layernorm_split", "rmem_dwconv5x5_split", "rmem_groupnorm2",
@@ -117,10 +154,12 @@ EXPORTS = [
     "rmem_bias_act_nchw_batched", "rmem_dwconv5x5_split2",
     "rmem_attn_read", "rmem_attn_read_trace", "rmem_attn_read2", "rmem_attn_read_combine", "rmem_attn_read_combine2",
     "rmem_rec_end", "rmem_launch_recorded", "rmem_groupnorm2_fold",
+    "rmem_bank8_plan", "rmem_bank8_append", "rmem_bank8_gather", "rmem_bank8_attn",
 ]
 # exports with a non-int return type
 EXPORTS_OTHER = ["rmem_rec_begin", "rmem_rec_free", "rmem_rec_count", "rmem_rec_size", "rmem_rec_data",
-                 "rmem_rec_signature"]
+                 "rmem_rec_signature", "rmem_bank8_attn_workspace",
+                 "rmem_bank8_append_workspace"]
 
 
 def lib_path() -> str:
@@ -143,6 +182,9 @@ def load():
     if lib.rmem_abi_version() != ABI_VERSION:
         raise RmemError(f"{_LIB_PATH} has ABI {lib.rmem_abi_version()}, this binding expects {ABI_VERSION}: "
                         "stale library -- rebuild with `python -m rmem_amd.build --force`")
+    for name in EXPORTS + EXPORTS_OTHER:
+        if not hasattr(lib, name):
+            raise RmemError(f"{_LIB_PATH} lacks {name}: stale library -- rebuild with `python -m rmem_amd.build --force`")
     for name in EXPORTS:
         getattr(lib, name).restype = C.c_int
     lib.rmem_configure.argtypes = [C.c_char_p, i64]
@@ -201,6 +243,12 @@ def load():
     lib.rmem_rec_data.restype, lib.rmem_rec_data.argtypes = c_p, [c_p]
     lib.rmem_rec_signature.restype, lib.rmem_rec_signature.argtypes = C.c_uint64, [c_p]
     lib.rmem_launch_recorded.argtypes = [c_p, c_p, i64, i32, c_p]
+    lib.rmem_bank8_plan.argtypes = [C.POINTER(Bank8PlanArgs), c_p]
+    lib.rmem_bank8_append.argtypes = [C.POINTER(Bank8AppendArgs), c_p]
+    lib.rmem_bank8_append_workspace.restype, lib.rmem_bank8_append_workspace.argtypes = i64, [C.POINTER(Bank8AppendArgs)]
+    lib.rmem_bank8_gather.argtypes = [C.POINTER(Bank8GatherArgs), c_p]
+    lib.rmem_bank8_attn.argtypes = [C.POINTER(Bank8AttnArgs), c_p]
+    lib.rmem_bank8_attn_workspace.restype, lib.rmem_bank8_attn_workspace.argtypes = i64, [C.POINTER(Bank8AttnArgs)]
     _LIB = lib
     _configure_from_environment(lib)
     return lib
