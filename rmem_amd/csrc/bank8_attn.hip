@@ -13,7 +13,11 @@
 // numbers below the maximum; fp32 calls keep them in two planes.  Sums are fp32, of the unrounded weights.
 #include "bank8.h"
 
+#include <type_traits>
+
 using namespace bank8;
+
+#define MFMA16(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0)
 
 namespace {
 
@@ -37,8 +41,15 @@ struct Req {
   int q0, n, len, rt, tiles;
 };
 
+// How a read is divided: `want` parts per kv head, none of fewer than `chunk_min` tiles, over the requests of `lo` .. `hi` rows per
+// kv head (a call may give short and long requests to different kernels).
+struct Split {
+  int G, ps, want, chunk_min;
+  int lo, hi;
+};
+
 template <int ROWS>
-__device__ __forceinline__ Req request(const rmem_bank8_attn_args& a, int r, int G) {
+__device__ __forceinline__ Req request(const rmem_bank8_attn_args& a, int r, const Split& sp) {
   Req x = {0, 0, 0, 0, 0};
   if (r >= a.reqs) return x;
   int q0 = a.cu[r], q1 = a.cu[r + 1], len = a.lens[r];
@@ -48,7 +59,8 @@ __device__ __forceinline__ Req request(const rmem_bank8_attn_args& a, int r, int
   x.q0 = q0;
   x.n = q1 - q0;
   x.len = len < 0 ? 0 : len > cap ? (int)cap : len;
-  x.rt = (int)(((long)x.n * G + ROWS - 1) / ROWS);
+  const long rows = (long)x.n * sp.G;
+  x.rt = rows < sp.lo || rows > sp.hi ? 0 : (int)((rows + ROWS - 1) / ROWS);
   x.tiles = (x.len + 31) >> 5;
   return x;
 }
@@ -64,21 +76,21 @@ __device__ __forceinline__ long wave_sum_long(long v) {
 
 // by_parts: index counts (request, row tile, part); otherwise (request, row tile) of requests in more than one part (the merge).
 template <int ROWS>
-__device__ bool find_unit(const rmem_bank8_attn_args& a, int G, long index, bool by_parts, int want, int chunk_min, Unit& u) {
+__device__ bool find_unit(const rmem_bank8_attn_args& a, const Split& sp, long index, bool by_parts, Unit& u) {
   const int lane = threadIdx.x & 63;
-  Req x = request<ROWS>(a, lane, G);
+  Req x = request<ROWS>(a, lane, sp);
   long total = (long)x.rt * x.tiles;
   for (int b = 64; b < a.reqs; b += 64) {
-    const Req y = request<ROWS>(a, b + lane, G);
+    const Req y = request<ROWS>(a, b + lane, sp);
     total += (long)y.rt * y.tiles;
   }
   total = wave_sum_long(total);
-  long chunk = (total + want - 1) / want;
-  chunk = chunk < chunk_min ? chunk_min : chunk;
+  total = (total + sp.want - 1) / sp.want;
+  const int chunk = total < sp.chunk_min ? sp.chunk_min : total > 0x3fffffff ? 0x3fffffff : (int)total;
   long seen = 0, slots = 0;
   for (int b = 0; b < a.reqs; b += 64) {
-    if (b) x = request<ROWS>(a, b + lane, G);
-    const int ns = x.tiles > chunk ? (int)((x.tiles + chunk - 1) / chunk) : 1;
+    if (b) x = request<ROWS>(a, b + lane, sp);
+    const int ns = x.tiles > chunk ? (x.tiles + chunk - 1) / chunk : 1;
     const int split = ns > 1 ? x.rt * ns : 0;
     int cnt = by_parts ? x.rt * ns : ns > 1 ? x.rt : 0;
     int c = cnt, s = split;
@@ -110,28 +122,101 @@ __device__ bool find_unit(const rmem_bank8_attn_args& a, int G, long index, bool
   return false;
 }
 
-// ------------------------------------------------------------------------------------------------------------ one key tile
-// Query fragments of one row: step 2 t + e covers dims 32 t + 16 hi + 8 e .. + 7, the order in which a lane's 16 key bytes lie.
-template <int D, int NS>
+// ---------------------------------------------------------------------------------------------------------- one token tile
+// Two shapes of the matrix instruction, by the rows of a tile (R).  `g` = lane / R is the lane's part of what its row's lanes share.
+//   R = 32 (32x32x16): S^T of 32 tokens in one product chain; lane (row, g) holds tokens (r & 3) + 8 (r >> 2) + 4 g in register r
+//   R = 16 (16x16x32): two chains of 16 tokens each; lane (row, g) holds tokens 16 (g & 1) + 4 (g >> 1) + (r & 3) + 8 (r >> 2),
+//          r = 0 .. 7: a group of up to 16 query heads on one token needs half the softmax arithmetic and half the registers
+// In both a lane's values in V^T's byte order are its P operand.
+template <int R>
+__device__ __forceinline__ float row_max(float x) {
+  float lo, up;
+  xor32_pair(x, lo, up);
+  x = fmaxf(lo, up);
+  if constexpr (R == 16) {
+    xor16_pair(x, lo, up);
+    x = fmaxf(lo, up);
+  }
+  return x;
+}
+template <int R>
+__device__ __forceinline__ float row_sum(float x) {
+  float lo, up;
+  xor32_pair(x, lo, up);
+  x = lo + up;
+  if constexpr (R == 16) {
+    xor16_pair(x, lo, up);
+    x = lo + up;
+  }
+  return x;
+}
+
+// Query fragments of one row.  A lane's 16 key bytes are 16 consecutive dims: chunk C t + g of 16 (C = 64 / R lanes per row), the
+// first 8 for step 2 t, the others for step 2 t + 1; with R = 16 and 32 dims a lane has 8 bytes, dims 8 g .. + 7, and one step.
+template <int R, int D, int NS>
 struct Query {
-  frag8_t f[NS][D / 16];
+  static constexpr int STEPS = R == 32 ? D / 16 : D / 32;
+  frag8_t f[NS][STEPS];
   float mul;               // scores' factor: softmax scale * log2 e / row's power of two
 };
 
-template <int D, int NS>
-__device__ __forceinline__ void load_query(Query<D, NS>& q, const void* p, long at, int type, bool on, int hi, float scale) {
-  float x[D / 32][16];
+template <int R, int D>
+__device__ __forceinline__ int step_dim(int step, int g) {
+  if (R == 16 && D == 32) return 8 * g;
+  return ((64 / R) * (step >> 1) + g) * 16 + 8 * (step & 1);
+}
+
+// one branch on type and alignment around all of a lane's loads: a branch per element makes each wait for the one before
+template <int R, int D, int S, class T>
+__device__ __forceinline__ void load_row(float (&x)[S][8], const T* p, int g, bool wide) {
+  typedef __attribute__((ext_vector_type(16 / sizeof(T)))) T vec_t;
+  constexpr int V = 16 / sizeof(T);
+  if (wide) {
+    vec_t y[S][8 / V];
+#pragma unroll
+    for (int t = 0; t < S; ++t)
+#pragma unroll
+      for (int k = 0; k < 8 / V; ++k) y[t][k] = *reinterpret_cast<const vec_t*>(p + step_dim<R, D>(t, g) + k * V);
+#pragma unroll
+    for (int t = 0; t < S; ++t)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[t][e] = (float)y[t][e / V][e % V];
+  } else {
+    T y[S][8];
+#pragma unroll
+    for (int t = 0; t < S; ++t)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[t][e] = p[step_dim<R, D>(t, g) + e];
+#pragma unroll
+    for (int t = 0; t < S; ++t)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[t][e] = (float)y[t][e];
+  }
+}
+
+template <int R, int D, int NS>
+__device__ __forceinline__ void load_query(Query<R, D, NS>& q, const rmem_bank8_attn_args& a, long row, int hq, bool on, int g) {
+  constexpr int S = Query<R, D, NS>::STEPS;
+  const int type = a.type;
+  const float scale = a.scale;
+  const long at = row * a.q_row + hq * a.q_head, es = type == FP32 ? 4 : 2;
+  const bool wide = (((unsigned long)a.q | (unsigned long)(a.q_row * es) | (unsigned long)(a.q_head * es)) & 15) == 0;
+  float x[S][8];
+#pragma unroll
+  for (int t = 0; t < S; ++t)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[t][e] = 0.f;
+  if (on) {
+    if constexpr (NS == 2) load_row<R, D>(x, static_cast<const float*>(a.q) + at, g, wide);
+    else if (type == FP16) load_row<R, D>(x, static_cast<const _Float16*>(a.q) + at, g, wide);
+    else load_row<R, D>(x, static_cast<const __bf16*>(a.q) + at, g, wide);
+  }
   float mx = 0.f;
 #pragma unroll
-  for (int t = 0; t < D / 32; ++t)
+  for (int t = 0; t < S; ++t)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      x[t][e] = on ? load1(p, at + 32 * t + 16 * hi + e, type) : 0.f;
-      mx = fmaxf(mx, fabsf(x[t][e]));
-    }
-  float lo, up;
-  xor32_pair(mx, lo, up);
-  mx = fmaxf(lo, up);
+    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[t][e]));
+  mx = row_max<R>(mx);
   // 2^(14 - exponent of the largest element), within fp32; rows of infinities are left as they are
   int e = 268 - (int)(__float_as_uint(mx) >> 23);
   e = e > 254 ? 254 : e;
@@ -140,88 +225,119 @@ __device__ __forceinline__ void load_query(Query<D, NS>& q, const void* p, long 
   q.mul = scale * LOG2E * __uint_as_float((unsigned)(254 - e) << 23);
   if (e == 254) q.mul = scale * LOG2E * 5.877471754e-39f;      // 2^-127
 #pragma unroll
-  for (int t = 0; t < D / 32; ++t)
+  for (int t = 0; t < S; ++t) {
+    frag8_t h, l;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      frag8_t h, l;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float y = x[t][8 * s + k] * f;
-        h[k] = (_Float16)y;
-        l[k] = (_Float16)(y - (float)h[k]);
-      }
-      q.f[0][2 * t + s] = h;
-      if constexpr (NS == 2) q.f[NS - 1][2 * t + s] = l;
+    for (int k = 0; k < 8; ++k) {
+      const float y = x[t][k] * f;
+      h[k] = (_Float16)y;
+      l[k] = (_Float16)(y - (float)h[k]);
     }
+    q.f[0][t] = h;
+    if constexpr (NS == 2) q.f[NS - 1][t] = l;
+  }
 }
 
-template <int D>
+// O^T of the lane's row, four consecutive dims at a time: quad i holds dims (256 / R) i + 4 g .. + 3
+template <int R, int D>
 struct Acc {
-  f32x16_t o[D / 32];
+  static constexpr int QUADS = D * R / 256, STRIDE = 256 / R;
+  typedef typename std::conditional<R == 32, f32x16_t, f32x4_t>::type tile_t;
+  tile_t o[D / R];
   float m, l;
+  __device__ __forceinline__ f32x4_t quad(int i) const {
+    if constexpr (R == 16) return o[i];
+    else {
+      const f32x4_t x = {o[i >> 2][4 * (i & 3)], o[i >> 2][4 * (i & 3) + 1], o[i >> 2][4 * (i & 3) + 2], o[i >> 2][4 * (i & 3) + 3]};
+      return x;
+    }
+  }
+  __device__ __forceinline__ void add(int i, f32x4_t x) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (R == 16) o[i][e] += x[e];
+      else o[i >> 2][4 * (i & 3) + e] += x[e];
+    }
+  }
+  __device__ __forceinline__ void mul(float f) {
+#pragma unroll
+    for (int d = 0; d < D / R; ++d)
+#pragma unroll
+      for (int r = 0; r < R / 2 * (R == 32) + 4 * (R == 16); ++r) o[d][r] *= f;
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int d = 0; d < D / R; ++d)
+#pragma unroll
+      for (int r = 0; r < R / 2 * (R == 32) + 4 * (R == 16); ++r) o[d][r] = 0.f;
+    m = LOWEST;
+    l = 0.f;
+  }
 };
 
-template <int D>
-__device__ __forceinline__ void clear(Acc<D>& c) {
-#pragma unroll
-  for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) c.o[d][r] = 0.f;
-  c.m = LOWEST;
-  c.l = 0.f;
-}
-
-// tokens tok0 .. tok0 + 31 against this lane's row, which sees tokens < lim; kf(step), vf(dim tile, step) give the fragments
-template <int D, int NS, class KF, class VF>
-__device__ __forceinline__ void tile(Acc<D>& c, const Query<D, NS>& q, int tok0, int lim, float ks, float lvs, float ivs, int hi, bool masked,
+// tokens tok0 .. tok0 + 31 against this lane's row, which sees tokens < lim; kf(step[, chain]), vf(dim tile[, step]) give fragments
+template <int R, int D, int NS, class KF, class VF>
+__device__ __forceinline__ void tile(Acc<R, D>& c, const Query<R, D, NS>& q, int tok0, int lim, float ks, float lvs, float ivs, int g, bool masked,
                                      KF kf, VF vf) {
-  f32x16_t s;
+  constexpr int N = R / 2;                  // tokens per lane
+  float s[N];
+  if constexpr (R == 32) {
+    f32x16_t x;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) s[r] = 0.f;
+    for (int r = 0; r < 16; ++r) x[r] = 0.f;
 #pragma unroll
-  for (int t = 0; t < D / 16; ++t) {
-    const frag8_t k = kf(t);
-    if constexpr (NS == 2) s = RMEM_MFMA(k, q.f[NS - 1][t], s);
-    s = RMEM_MFMA(k, q.f[0][t], s);
+    for (int t = 0; t < D / 16; ++t) {
+      const frag8_t k = kf(t, 0);
+      if constexpr (NS == 2) x = RMEM_MFMA(k, q.f[NS - 1][t], x);
+      x = RMEM_MFMA(k, q.f[0][t], x);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = x[r];
+  } else {
+    f32x4_t x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const frag8_t f = kf(t, k);
+        if constexpr (NS == 2) x[k] = MFMA16(f, q.f[NS - 1][t], x[k]);
+        x[k] = MFMA16(f, q.f[0][t], x[k]);
+      }
+#pragma unroll
+    for (int r = 0; r < 8; ++r) s[r] = x[r >> 2][r & 3];
   }
   const float mul = q.mul * ks;
   float top;
-  const int left = lim - tok0 - 4 * hi;      // register r holds token tok0 + 4 hi + (r & 3) + 8 (r >> 2)
+  const int left = lim - tok0 - (R == 32 ? 4 * g : 16 * (g & 1) + 4 * (g >> 1));   // register r holds token (r & 3) + 8 (r >> 2) of these
   if (!masked) {
     top = s[0];
 #pragma unroll
-    for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+    for (int r = 1; r < N; ++r) top = fmaxf(top, s[r]);
     top = fmaf(top, mul, lvs);
   } else {
     top = LOWEST;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) top = fmaxf(top, (r & 3) + 8 * (r >> 2) < left ? fmaf(s[r], mul, lvs) : LOWEST);
+    for (int r = 0; r < N; ++r) top = fmaxf(top, (r & 3) + 8 * (r >> 2) < left ? fmaf(s[r], mul, lvs) : LOWEST);
   }
-  float lo, up;
-  xor32_pair(top, lo, up);
-  const float m = fmaxf(c.m, fmaxf(lo, up));
+  const float m = fmaxf(c.m, row_max<R>(top));
   const float add = lvs - m + LIFT;
-  float w[16], sum = 0.f;
+  float w[N], sum = 0.f;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
+  for (int r = 0; r < N; ++r) {
     w[r] = __builtin_amdgcn_exp2f(fmaf(s[r], mul, add));
     if (masked) w[r] = (r & 3) + 8 * (r >> 2) < left ? w[r] : 0.f;
     sum += w[r];
   }
-  xor32_pair(sum, lo, up);
-  sum = (lo + up) * ivs;
+  sum = row_sum<R>(sum) * ivs;
   if (__any(m != c.m)) {
     const float alpha = __builtin_amdgcn_exp2f(c.m - m);
     c.l *= alpha;
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) c.o[d][r] *= alpha;
+    c.mul(alpha);
     c.m = m;
   }
   c.l += sum;
 #pragma unroll
-  for (int st = 0; st < 2; ++st) {
+  for (int st = 0; st < N / 8; ++st) {
     frag8_t p, pl;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -229,48 +345,42 @@ __device__ __forceinline__ void tile(Acc<D>& c, const Query<D, NS>& q, int tok0,
       if constexpr (NS == 2) pl[e] = (_Float16)(w[8 * st + e] - (float)p[e]);
     }
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d) {
+    for (int d = 0; d < D / R; ++d) {
       const frag8_t v = vf(d, st);
-      if constexpr (NS == 2) c.o[d] = RMEM_MFMA(v, pl, c.o[d]);
-      c.o[d] = RMEM_MFMA(v, p, c.o[d]);
+      if constexpr (R == 32) {
+        if constexpr (NS == 2) c.o[d] = RMEM_MFMA(v, pl, c.o[d]);
+        c.o[d] = RMEM_MFMA(v, p, c.o[d]);
+      } else {
+        if constexpr (NS == 2) c.o[d] = MFMA16(v, pl, c.o[d]);
+        c.o[d] = MFMA16(v, p, c.o[d]);
+      }
     }
   }
 }
 
-// e4m3 bytes behind the request's last token may be NaN, and 0 * NaN is not 0: words m of a lane's 16 value bytes hold tokens
-// 8 m + 4 hi .. + 3 of the tile
-__device__ __forceinline__ u32x4_t keep_first(u32x4_t v, int valid, int hi) {
-#pragma unroll
-  for (int m = 0; m < 4; ++m) {
-    const int n = valid - 8 * m - 4 * hi;
-    v[m] = n >= 4 ? v[m] : n <= 0 ? 0u : v[m] & ((1u << (8 * n)) - 1u);
-  }
-  return v;
-}
+// the first n of a word's four bytes
+__device__ __forceinline__ uint32_t keep_first(uint32_t v, int n) { return n >= 4 ? v : n <= 0 ? 0u : v & ((1u << (8 * n)) - 1u); }
 
 __device__ __forceinline__ float readlane(float x, int l) {
   return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), l));
 }
 
 // ------------------------------------------------------------------------------------------------------------ result rows
-__device__ __forceinline__ void store4(void* p, long at, float a, float b, float c, float d, int type, bool wide) {
-  if (!wide) {
-    store1(p, at, a, type);
-    store1(p, at + 1, b, type);
-    store1(p, at + 2, c, type);
-    store1(p, at + 3, d, type);
-  } else if (type == FP32) {
-    const f32x4_t w = {a, b, c, d};
-    *reinterpret_cast<f32x4_t*>(static_cast<float*>(p) + at) = w;
-  } else if (type == FP16) {
-    typedef __attribute__((ext_vector_type(4))) _Float16 h4;
-    const h4 w = {(_Float16)a, (_Float16)b, (_Float16)c, (_Float16)d};
-    *reinterpret_cast<h4*>(static_cast<_Float16*>(p) + at) = w;
-  } else {
-    typedef __attribute__((ext_vector_type(4))) __bf16 b4;
-    const b4 w = {(__bf16)a, (__bf16)b, (__bf16)c, (__bf16)d};
-    *reinterpret_cast<b4*>(static_cast<__bf16*>(p) + at) = w;
+template <class T>
+__device__ __forceinline__ void store4(T* p, f32x4_t x, bool wide) {
+  typedef __attribute__((ext_vector_type(4))) T vec_t;
+  const vec_t w = {(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
+  if (wide) *reinterpret_cast<vec_t*>(p) = w;
+  else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) p[e] = w[e];
   }
+}
+template <class F>
+__device__ __forceinline__ void by_type(int type, void* p, F f) {
+  if (type == FP32) f(static_cast<float*>(p));
+  else if (type == FP16) f(static_cast<_Float16*>(p));
+  else f(static_cast<__bf16*>(p));
 }
 
 __device__ __forceinline__ bool wide_stores(const rmem_bank8_attn_args& a) {
@@ -278,19 +388,16 @@ __device__ __forceinline__ bool wide_stores(const rmem_bank8_attn_args& a) {
   return (((unsigned long)a.out | (unsigned long)(a.o_row * es) | (unsigned long)(a.o_head * es)) & (4 * es - 1)) == 0;
 }
 
-// a lane's share of its row: registers 4 k .. 4 k + 3 of tile d are dims 32 d + 8 k + 4 hi .. + 3
-template <int D>
-__device__ __forceinline__ void write_row(const rmem_bank8_attn_args& a, const Acc<D>& c, int hq, long row, int hi) {
+template <int R, int D>
+__device__ __forceinline__ void write_row(const rmem_bank8_attn_args& a, const Acc<R, D>& c, int hq, long row, int g) {
   const float inv = c.l > 0.f ? 1.0f / c.l : c.l != c.l ? c.l : 0.f;
   const bool wide = wide_stores(a);
   const long at = row * a.o_row + hq * a.o_head;
+  by_type(a.type, a.out, [&](auto* p) {
 #pragma unroll
-  for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      store4(a.out, at + 32 * d + 8 * k + 4 * hi, c.o[d][4 * k] * inv, c.o[d][4 * k + 1] * inv, c.o[d][4 * k + 2] * inv, c.o[d][4 * k + 3] * inv,
-             a.type, wide);
-  if (a.lse && hi == 0) a.lse[row * a.heads_q + hq] = (__log2f(c.l) + c.m - LIFT) * LN2;
+    for (int i = 0; i < Acc<R, D>::QUADS; ++i) store4(p + at + Acc<R, D>::STRIDE * i + 4 * g, c.quad(i) * inv, wide);
+  });
+  if (a.lse && g == 0) a.lse[row * a.heads_q + hq] = (__log2f(c.l) + c.m - LIFT) * LN2;
 }
 
 // partial results of split units: [slot][kv head][ROWS][D] fp32, then [slot][kv head][ROWS][2] (maximum, sum)
@@ -300,47 +407,121 @@ struct Parts {
   int slots;              // units that fit
 };
 
-template <int D, int ROWS>
-__device__ __forceinline__ void write_part(const Parts& w, const Acc<D>& c, int slot, int h, int heads, int j, int hi) {
+template <int ROWS, int R, int D>
+__device__ __forceinline__ void write_part(const Parts& w, const Acc<R, D>& c, int slot, int h, int heads, int j, int g) {
   const long row = ((long)slot * heads + h) * ROWS + j;
 #pragma unroll
-  for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const f32x4_t x = {c.o[d][4 * k], c.o[d][4 * k + 1], c.o[d][4 * k + 2], c.o[d][4 * k + 3]};
-      *reinterpret_cast<f32x4_t*>(w.o + row * D + 32 * d + 8 * k + 4 * hi) = x;
-    }
-  if (hi == 0) {
+  for (int i = 0; i < Acc<R, D>::QUADS; ++i) *reinterpret_cast<f32x4_t*>(w.o + row * D + Acc<R, D>::STRIDE * i + 4 * g) = c.quad(i);
+  if (g == 0) {
     w.ml[row * 2] = c.m;
     w.ml[row * 2 + 1] = c.l;
   }
 }
 
 // ------------------------------------------------------------------------------------------------------- few rows per head
-// Four waves share a unit of 32 rows: wave w takes token tiles w, w + 4, ..., straight from memory into operand registers, the
+// Four waves share a unit of R rows: wave w takes token tiles w, w + 4, ..., straight from memory into operand registers, the
 // next tile's loads in flight behind the present one's arithmetic; the four partial results are joined through LDS.
 // Page ids and scales of a wave's next 64 tiles sit one per lane.
-template <int D, int CODE, int NS>
-__global__ __launch_bounds__(256, 2) void attn_narrow(rmem_bank8_attn_args a, Parts parts, int G, int ps, int want, int chunk_min) {
-  constexpr int DT = D / 32;
-  __shared__ __attribute__((aligned(16))) f32x4_t s_o[2][DT * 4][64];
+template <int R, int D>
+struct Raw;                               // a lane's codes of a tile
+template <int D>
+struct Raw<32, D> {
+  u32x4_t k[D / 32], v[D / 32];
+  __device__ __forceinline__ void load(const uint8_t* kp, const uint8_t* vp, int page, int j, int g) {
+    const unsigned ko = (unsigned)(g * page + j) * 16u, vo = (unsigned)(g * D + j) * 16u;
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) k[t] = *reinterpret_cast<const u32x4_t*>(kp + ko + (unsigned)(t * page) * 32u);
+    asm volatile("" ::: "memory");          // keys are wanted first: loads return in the order of their issue
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) v[t] = *reinterpret_cast<const u32x4_t*>(vp + vo + t * 512u);
+  }
+  // e4m3 bytes behind the request's last token may be NaN, and 0 * NaN is not 0
+  __device__ __forceinline__ void cut(int valid, int g) {
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+      for (int m = 0; m < 4; ++m) v[t][m] = keep_first(v[t][m], valid - 8 * m - 4 * g);
+  }
+  template <int CODE>
+  __device__ __forceinline__ frag8_t kf(int t, int) const { return decode8<CODE>(k[t >> 1][2 * (t & 1)], k[t >> 1][2 * (t & 1) + 1]); }
+  template <int CODE>
+  __device__ __forceinline__ frag8_t vf(int d, int st) const { return decode8<CODE>(v[d][2 * st], v[d][2 * st + 1]); }
+};
+template <int D>
+struct Raw<16, D> {
+  static constexpr int KC = D == 32 ? 1 : D / 64;      // 16-byte (32 dims: 8-byte) loads per token
+  u32x4_t k[2][KC];
+  u32x2_t v[D / 16];
+  __device__ __forceinline__ void load(const uint8_t* kp, const uint8_t* vp, int page, int j, int g) {
+    const int tok = 4 * (j >> 3) + 16 * ((j >> 2) & 1) + (j & 3);    // of chain 0, row j of S^T; chain 1: 8 further on
+    if constexpr (D == 32) {
+      const unsigned ko = (unsigned)((g >> 1) * page + tok) * 16u + 8u * (g & 1);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const u32x2_t x = *reinterpret_cast<const u32x2_t*>(kp + ko + c * 128u);
+        k[c][0][0] = x[0];
+        k[c][0][1] = x[1];
+      }
+    } else {
+      const unsigned ko = (unsigned)(g * page + tok) * 16u;
+#pragma unroll
+      for (int t = 0; t < KC; ++t)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) k[c][t] = *reinterpret_cast<const u32x4_t*>(kp + ko + (unsigned)(t * page) * 64u + c * 128u);
+    }
+    asm volatile("" ::: "memory");          // keys are wanted first: loads return in the order of their issue
+    const unsigned vo = (unsigned)((g >> 1) * D + j) * 16u + 8u * (g & 1);
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) v[d] = *reinterpret_cast<const u32x2_t*>(vp + vo + d * 256u);
+  }
+  __device__ __forceinline__ void cut(int valid, int g) {
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+      for (int m = 0; m < 2; ++m) v[d][m] = keep_first(v[d][m], valid - 8 * m - 16 * (g & 1) - 4 * (g >> 1));
+  }
+  template <int CODE>
+  __device__ __forceinline__ frag8_t kf(int t, int c) const {
+    if constexpr (D == 32) return decode8<CODE>(k[c][0][0], k[c][0][1]);
+    else return decode8<CODE>(k[c][t >> 1][2 * (t & 1)], k[c][t >> 1][2 * (t & 1) + 1]);
+  }
+  template <int CODE>
+  __device__ __forceinline__ frag8_t vf(int d, int) const { return decode8<CODE>(v[d][0], v[d][1]); }
+};
+
+// ROWS rows of a unit from first_row on: sees = tokens seen by some of them, all = by every one
+struct Sees {
+  int sees, all;
+};
+template <int ROWS>
+__device__ __forceinline__ Sees rows_see(const Unit& u, int first_row, int causal, int G) {
+  const int first = first_row / G, last = min(u.n - 1, (first_row + ROWS - 1) / G);
+  Sees x;
+  x.sees = first >= u.n ? 0 : max(0, causal ? u.len - u.n + last + 1 : u.len);
+  x.all = max(0, causal ? u.len - u.n + first + 1 : u.len);
+  return x;
+}
+
+template <int R, int D, int CODE, int NS>
+__global__ __launch_bounds__(256, 2) void attn_narrow(rmem_bank8_attn_args a, Parts parts, Split sp) {
+  const int G = sp.G, ps = sp.ps;
+  constexpr int QUADS = Acc<R, D>::QUADS;
+  __shared__ __attribute__((aligned(16))) f32x4_t s_o[2][QUADS][64];
   __shared__ float s_m[4][64], s_l[4][64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, j = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, g = lane / R, j = lane % R;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);       // uniform: tile counts and page addresses stay scalar
   const int heads = a.bank.heads, h = blockIdx.x % heads;
   Unit u;
-  if (!find_unit<32>(a, G, blockIdx.x / heads, true, want, chunk_min, u)) return;
-  const int row = u.rt * 32 + j, qt = row / G, hq = h * G + row % G;
+  if (!find_unit<R>(a, sp, blockIdx.x / heads, true, u)) return;
+  const int row = u.rt * R + j, qt = row / G, hq = h * G + row % G;
   const bool on = qt < u.n;
   const int lim = !on ? 0 : a.causal ? min(u.len, u.len - u.n + qt + 1) : u.len;     // may be <= 0
-  // tokens that the tile's last row sees, and this part of them
-  const int last = min(u.n - 1, (u.rt * 32 + 31) / G);
-  const int sees = max(0, a.causal ? u.len - u.n + last + 1 : u.len);
-  const int first = max(0, a.causal ? u.len - u.n + u.rt * 32 / G + 1 : u.len);     // seen by every row of the tile
-  const int tiles = (sees + 31) >> 5, per = (tiles + u.ns - 1) / u.ns;
+  const Sees see = rows_see<R>(u, u.rt * R, a.causal, G);
+  const int tiles = (see.sees + 31) >> 5, per = (tiles + u.ns - 1) / u.ns;
   const int t0 = u.part * per, t1 = min(tiles, t0 + per);
 
-  Query<D, NS> q;
-  load_query<D, NS>(q, a.q, (long)(u.q0 + qt) * a.q_row + (long)hq * a.q_head, a.type, on, hi, a.scale);
+  Query<R, D, NS> q;
+  load_query<R, D, NS>(q, a, u.q0 + qt, hq, on, g);
 
   const int page = a.bank.page;
   const long block = (long)page * D;        // bytes of one (page, head)
@@ -348,11 +529,10 @@ __global__ __launch_bounds__(256, 2) void attn_narrow(rmem_bank8_attn_args a, Pa
   const uint8_t* kb = a.bank.k + h * block;
   const uint8_t* vb = a.bank.v + h * block;
   const long pstride = heads * block;
-  const unsigned koff = (unsigned)(hi * page + j) * 16u, kstep = (unsigned)page * 32u, voff = (unsigned)(hi * D + j) * 16u;
   const int sub_mask = (1 << (ps - 5)) - 1;
 
-  Acc<D> c;
-  clear(c);
+  Acc<R, D> c;
+  c.clear();
   for (int base = t0 + wave; base < t1; base += 256) {
     const int nt = min(64, (t1 - base + 3) >> 2);
     int pid = -1;
@@ -366,36 +546,30 @@ __global__ __launch_bounds__(256, 2) void attn_narrow(rmem_bank8_attn_args a, Pa
       }
     }
     const float lvs = __log2f(vs), ivs = 1.0f / vs;
-    u32x4_t kr[2][DT], vr[2][DT];
-    auto load = [&](int i, u32x4_t* k, u32x4_t* v) __attribute__((always_inline)) {
+    Raw<R, D> raw[2];
+    auto load = [&](int i, Raw<R, D>& x) __attribute__((always_inline)) {
       const int id = __builtin_amdgcn_readlane(pid, i), sub = (base + 4 * i) & sub_mask;
       const long at = (id < 0 ? 0 : id) * pstride;
-      const uint8_t* kp = kb + at + (unsigned)sub * 512u;
-      const uint8_t* vp = vb + at + (unsigned)sub * (32u * D);
-#pragma unroll
-      for (int t = 0; t < DT; ++t) k[t] = *reinterpret_cast<const u32x4_t*>(kp + koff + t * kstep);
-#pragma unroll
-      for (int t = 0; t < DT; ++t) v[t] = *reinterpret_cast<const u32x4_t*>(vp + voff + t * 512u);
+      x.load(kb + at + (unsigned)sub * 512u, vb + at + (unsigned)sub * (32u * D), page, j, g);
     };
-    auto step = [&](int i, u32x4_t* k, u32x4_t* v) __attribute__((always_inline)) {
+    auto step = [&](int i, Raw<R, D>& x) __attribute__((always_inline)) {
       const int tok0 = (base + 4 * i) * 32;
       const bool absent = __builtin_amdgcn_readlane(pid, i) < 0;
       const int end = absent ? tok0 : u.len;
-      if (CODE == E4M3 && tok0 + 32 > end) {
-#pragma unroll
-        for (int t = 0; t < DT; ++t) v[t] = keep_first(v[t], end - tok0, hi);
-      }
-      tile<D, NS>(c, q, tok0, min(lim, end), readlane(ks, i), readlane(lvs, i), readlane(ivs, i), hi, tok0 + 32 > min(first, end),
-                  [&](int t) { return decode8<CODE>(k[t >> 1][2 * (t & 1)], k[t >> 1][2 * (t & 1) + 1]); },
-                  [&](int d, int st) { return decode8<CODE>(v[d][2 * st], v[d][2 * st + 1]); });
+      if (CODE == E4M3 && tok0 + 32 > end) x.cut(end - tok0, g);
+      tile<R, D, NS>(c, q, tok0, min(lim, end), readlane(ks, i), readlane(lvs, i), readlane(ivs, i), g, tok0 + 32 > min(see.all, end),
+                     [&](int t, int k) { return x.template kf<CODE>(t, k); }, [&](int d, int st) { return x.template vf<CODE>(d, st); });
     };
-    load(0, kr[0], vr[0]);
-    for (int i = 0; i < nt; i += 2) {
-      if (i + 1 < nt) load(i + 1, kr[1], vr[1]);
-      step(i, kr[0], vr[0]);
+    // The loads are unconditional (the last tile again where there is no next one): with a way around them the compiler would have
+    // to wait for all that may be in flight before it touches the present tile.
+    load(0, raw[0]);
+    for (int i = 0;; i += 2) {
+      load(min(i + 1, nt - 1), raw[1]);
+      step(i, raw[0]);
       if (i + 1 >= nt) break;
-      if (i + 2 < nt) load(i + 2, kr[0], vr[0]);
-      step(i + 1, kr[1], vr[1]);
+      load(min(i + 2, nt - 1), raw[0]);
+      step(i + 1, raw[1]);
+      if (i + 2 >= nt) break;
     }
   }
 
@@ -407,31 +581,16 @@ __global__ __launch_bounds__(256, 2) void attn_narrow(rmem_bank8_attn_args a, Pa
   float l = 0.f;
 #pragma unroll
   for (int w = 0; w < 4; ++w) l += s_l[w][lane] * __builtin_amdgcn_exp2f(s_m[w][lane] - m);
-  const float alpha = __builtin_amdgcn_exp2f(c.m - m);
-#pragma unroll
-  for (int d = 0; d < DT; ++d)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) c.o[d][r] *= alpha;
+  c.mul(__builtin_amdgcn_exp2f(c.m - m));
   c.m = m;
   c.l = l;
   auto put = [&](int to) __attribute__((always_inline)) {
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const f32x4_t x = {c.o[d][4 * k], c.o[d][4 * k + 1], c.o[d][4 * k + 2], c.o[d][4 * k + 3]};
-        s_o[to][d * 4 + k][lane] = x;
-      }
+    for (int i = 0; i < QUADS; ++i) s_o[to][i][lane] = c.quad(i);
   };
   auto get = [&](int from) __attribute__((always_inline)) {
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const f32x4_t x = s_o[from][d * 4 + k][lane];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c.o[d][4 * k + e] += x[e];
-      }
+    for (int i = 0; i < QUADS; ++i) c.add(i, s_o[from][i][lane]);
   };
   if (wave >= 2) put(wave - 2);
   __syncthreads();
@@ -442,60 +601,217 @@ __global__ __launch_bounds__(256, 2) void attn_narrow(rmem_bank8_attn_args a, Pa
   if (wave != 0) return;
   get(0);
   if (!on) return;
-  if (u.ns == 1) write_row<D>(a, c, hq, u.q0 + qt, hi);
-  else if (u.slot + u.part < parts.slots) write_part<D, 32>(parts, c, u.slot + u.part, h, heads, j, hi);
+  if (u.ns == 1) write_row<R, D>(a, c, hq, u.q0 + qt, g);
+  else if (u.slot + u.part < parts.slots) write_part<R, R, D>(parts, c, u.slot + u.part, h, heads, j, g);
+}
+
+// ------------------------------------------------------------------------------------------------------ many rows per head
+// Four waves of 32 rows each share a unit's tokens, 64 at a time: codes come through registers (the next stage's loads in flight
+// during this stage's arithmetic), are decoded once per workgroup and lie in LDS as fp16 fragments, in the order in which the
+// waves read them: 16 bytes per lane, contiguous.  Two buffers, one barrier per stage.
+// Decoding ahead of LDS costs a wave a quarter of the conversions and doubles the LDS bytes: at 128 dims a wave reads 16 KB per 32
+// tokens, 512 clocks for four waves at 128 B per clock, as long as their matrix instructions; decoding behind it would put 128
+// conversions per 32 tokens beside every wave's softmax arithmetic, which is the longer pipe.
+constexpr int WROWS = 128;
+
+template <int D, int CODE, int NS>
+__global__ __launch_bounds__(256, 2) void attn_wide(rmem_bank8_attn_args a, Parts parts, Split sp) {
+  constexpr int R = 32, CH = D / 32;             // 16-byte chunks per thread and stage: 8 D / 256
+  constexpr int HALF = 64 * D / 8;               // fragments (16 bytes) of a stage's keys; as many of its values
+  __shared__ __attribute__((aligned(16))) u32x4_t s_kv[2][2 * HALF];
+  const int G = sp.G, ps = sp.ps;
+  const int tid = threadIdx.x, lane = tid & 63, g = lane / R, j = lane % R;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int heads = a.bank.heads, h = blockIdx.x % heads;
+  Unit u;
+  if (!find_unit<WROWS>(a, sp, blockIdx.x / heads, true, u)) return;
+  const int row0 = u.rt * WROWS + wave * R, row = row0 + j, qt = row / G, hq = h * G + row % G;
+  const bool on = qt < u.n;
+  const int lim = !on ? 0 : a.causal ? min(u.len, u.len - u.n + qt + 1) : u.len;
+  const Sees see = rows_see<R>(u, row0, a.causal, G);                        // this wave's rows
+  const int tiles = (rows_see<WROWS>(u, u.rt * WROWS, a.causal, G).sees + 31) >> 5, per = (tiles + u.ns - 1) / u.ns;
+  const int t0 = u.part * per, t1 = min(tiles, t0 + per), stages = (t1 - t0 + 1) >> 1;
+
+  Query<R, D, NS> q;
+  load_query<R, D, NS>(q, a, u.q0 + qt, hq, on, g);
+
+  const int page = a.bank.page;
+  const long block = (long)page * D;
+  const int32_t* table = a.table + (long)u.r * a.ld_table;
+  const uint8_t* kb = a.bank.k + h * block;
+  const uint8_t* vb = a.bank.v + h * block;
+  const long pstride = heads * block;
+  const int sub_mask = (1 << (ps - 5)) - 1;
+
+  // page of tile t0 + 64 c + lane; -1: none
+  auto pages_of = [&](int c) __attribute__((always_inline)) {
+    const int t = t0 + 64 * c + lane;
+    int id = -1;
+    if (t < t1) id = table[t >> (ps - 5)];
+    return id < a.bank.pages ? id : -1;
+  };
+  u32x4_t raw[CH];
+  int page0 = -1, page1 = -1;                    // pages of the two tiles in `raw`
+  int load_pid = -1;                             // pages of the 64 tiles around them
+  auto load = [&](int st) __attribute__((always_inline)) {
+    if ((st & 31) == 0) load_pid = pages_of(st >> 5);
+    const int i = (2 * st) & 63, ta = t0 + 2 * st;
+    page0 = __builtin_amdgcn_readlane(load_pid, i);
+    page1 = __builtin_amdgcn_readlane(load_pid, i + 1);
+    const long a0 = (page0 < 0 ? 0 : page0) * pstride, a1 = (page1 < 0 ? 0 : page1) * pstride;
+    const int s0 = ta & sub_mask, s1 = (ta + 1) & sub_mask;
+#pragma unroll
+    for (int it = 0; it < CH; ++it) {
+      const int c = it * 256 + tid;
+      const uint8_t* p;
+      if (it * 256 + wave * 64 < 4 * D) {        // keys: a wave takes the 64 tokens of 16 dims
+        const int tok = c & 63, cc = c >> 6;
+        p = kb + (tok < 32 ? a0 + s0 * 512 : a1 + s1 * 512) + (unsigned)(cc * page + (tok & 31)) * 16u;
+      } else {                                   // values: dims of half th & 1 of tile th >> 1, the same tile for a wave
+        const int v = c - 4 * D, d = v % D, th = v / D;
+        p = vb + (__builtin_amdgcn_readfirstlane(th >> 1) ? a1 + s1 * (32 * D) : a0 + s0 * (32 * D)) + (unsigned)((th & 1) * D + d) * 16u;
+      }
+      raw[it] = *reinterpret_cast<const u32x4_t*>(p);
+    }
+  };
+  auto put = [&](int st, u32x4_t* to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int it = 0; it < CH; ++it) {
+      const int c = it * 256 + tid;
+      u32x4_t x = raw[it];
+      int at;
+      if (it * 256 + wave * 64 < 4 * D) {
+        const int tok = c & 63, cc = c >> 6;
+        at = ((((tok >> 5) * (D / 16) + (cc & ~1)) * 2 + (cc & 1)) << 5) + (tok & 31);
+      } else {
+        const int v = c - 4 * D, d = v % D, th = v / D;
+        at = HALF + ((((th >> 1) * (D / 32) + (d >> 5)) * 4 + (th & 1)) << 5) + (d & 31);
+        if constexpr (CODE == E4M3) {            // NaN codes behind the last token
+          const int sub = __builtin_amdgcn_readfirstlane(th >> 1), left = u.len - (t0 + 2 * st + sub) * 32;
+          if (left < 32) {
+#pragma unroll
+            for (int m = 0; m < 4; ++m) x[m] = keep_first(x[m], left - 8 * m - 4 * (th & 1));
+          }
+        }
+      }
+      to[at] = __builtin_bit_cast(u32x4_t, decode8<CODE>(x[0], x[1]));
+      to[at + 64] = __builtin_bit_cast(u32x4_t, decode8<CODE>(x[2], x[3]));
+    }
+  };
+
+  Acc<R, D> c;
+  c.clear();
+  int pid = -1;                                  // pages and scales of 64 tiles, one per lane
+  float ks = 0.f, lvs = 0.f, ivs = 1.f;
+  if (stages > 0) {
+    load(0);
+    put(0, s_kv[0]);
+    load(min(1, stages - 1));
+  }
+  for (int st = 0; st < stages; ++st) {
+    if ((st & 31) == 0) {
+      pid = pages_of(st >> 5);
+      float vs = 1.f;
+      if (pid >= 0) {
+        ks = a.bank.k_scale[(long)pid * heads + h];
+        vs = fmaxf(a.bank.v_scale[(long)pid * heads + h], VS_MIN);
+      }
+      lvs = __log2f(vs);
+      ivs = 1.0f / vs;
+    }
+    __syncthreads();                             // stage st is in its buffer, and every wave is done with the other one
+    if (st + 1 < stages) put(st + 1, s_kv[(st + 1) & 1]);
+    if (st + 2 < stages) load(st + 2);
+    const u32x4_t* kv = s_kv[st & 1];
+#pragma unroll 1
+    for (int sub = 0; sub < 2; ++sub) {
+      const int t = t0 + 2 * st + sub, i = (2 * st + sub) & 63, tok0 = t * 32;
+      if (t >= t1 || tok0 >= see.sees || __builtin_amdgcn_readlane(pid, i) < 0) continue;
+      tile<R, D, NS>(c, q, tok0, lim, readlane(ks, i), readlane(lvs, i), readlane(ivs, i), g, tok0 + 32 > min(see.all, u.len),
+                     [&](int k, int) { return __builtin_bit_cast(frag8_t, kv[(sub * (D / 16) + k) * 64 + lane]); },
+                     [&](int d, int k) { return __builtin_bit_cast(frag8_t, kv[HALF + ((sub * (D / 32) + d) * 2 + k) * 64 + lane]); });
+    }
+  }
+  if (!on) return;
+  if (u.ns == 1) write_row<R, D>(a, c, hq, u.q0 + qt, g);
+  else if (u.slot + u.part < parts.slots) write_part<WROWS, R, D>(parts, c, u.slot + u.part, h, heads, wave * R + j, g);
 }
 
 // ------------------------------------------------------------------------------------------------------------------- merge
-// One workgroup per (row tile of a split request, kv head, row): the parts of a row in order, D / 4 threads per part.
-template <int ROWS>
-__global__ __launch_bounds__(256) void attn_merge(rmem_bank8_attn_args a, Parts parts, int G, int want, int chunk_min) {
-  __shared__ f32x4_t s_o[256];
-  const int D = a.bank.dim, heads = a.bank.heads, tid = threadIdx.x;
-  const int h = blockIdx.x % heads, j = blockIdx.y;
+// One wave per (row tile of a split request, kv head, row): D / 4 lanes per part, the row's parts in order over the 256 / D groups
+// of lanes.  Waves of their own so that one round of them fills the chip: most of a call's grid finds nothing to do.
+template <int D>
+__device__ __forceinline__ float over_groups(float x) {       // sum over the lanes that hold the same dims
+  x += xor_lane<32>(x);
+  if constexpr (D <= 64) x += xor_lane<16>(x);
+  if constexpr (D <= 32) x += xor_lane<8>(x);
+  return x;
+}
+template <int ROWS, int D>
+__global__ __launch_bounds__(64) void attn_merge(rmem_bank8_attn_args a, Parts parts, Split sp) {
+  const int heads = a.bank.heads, lane = threadIdx.x, G = sp.G;
+  const int h = blockIdx.x % heads;
   Unit u;
-  if (!find_unit<ROWS>(a, G, blockIdx.x / heads, false, want, chunk_min, u)) return;
-  const int row = u.rt * ROWS + j, qt = row / G, hq = h * G + row % G;
-  if (qt >= u.n || u.slot + u.ns > parts.slots) return;
-  const long first = ((long)u.slot * heads + h) * ROWS + j, step = (long)heads * ROWS;
-  float m = LOWEST;
-  for (int p = tid & 63; p < u.ns; p += 64) m = fmaxf(m, parts.ml[(first + p * step) * 2]);
-  m = wave_max_xor(m);
-  const int width = D / 4, groups = 256 / width, g = tid / width, d4 = tid % width;
-  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
-  for (int p = g; p < u.ns; p += groups) {
-    const long at = first + p * step;
-    const float f = __builtin_amdgcn_exp2f(parts.ml[at * 2] - m);
-    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(parts.o + at * D + d4 * 4);
+  if (!find_unit<ROWS>(a, sp, blockIdx.x / heads, false, u)) return;
+  if (u.slot + u.ns > parts.slots) return;
+  constexpr int WIDTH = D / 4, GROUPS = 64 / WIDTH;
+  const int g = lane / WIDTH, d4 = lane % WIDTH;
+  const bool wide = wide_stores(a);
+  for (int j = blockIdx.y; j < ROWS; j += gridDim.y) {
+    const int row = u.rt * ROWS + j, qt = row / G, hq = h * G + row % G;
+    if (qt >= u.n) break;
+    const long first = ((long)u.slot * heads + h) * ROWS + j, step = (long)heads * ROWS;
+    float m = LOWEST;
+    for (int p = lane; p < u.ns; p += 64) m = fmaxf(m, parts.ml[(first + p * step) * 2]);
+    m = wave_max_xor(m);
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f;
+#pragma unroll 8
+    for (int p = g; p < u.ns; p += GROUPS) {
+      const long at = first + p * step;
+      const float f = __builtin_amdgcn_exp2f(parts.ml[at * 2] - m);
+      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(parts.o + at * D + d4 * 4);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
-    l = fmaf(parts.ml[at * 2 + 1], f, l);
-  }
-  __shared__ float s_l[32];
-  s_o[tid] = o;
-  if (d4 == 0) s_l[g] = l;
-  __syncthreads();
-  if (g) return;
-  for (int k = 1; k < groups; ++k) {
-    const f32x4_t x = s_o[k * width + d4];
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
+      l = fmaf(parts.ml[at * 2 + 1], f, l);
+    }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] += x[e];
-    l += s_l[k];
+    for (int e = 0; e < 4; ++e) o[e] = over_groups<D>(o[e]);
+    l = over_groups<D>(l);
+    if (g) continue;
+    const float inv = l > 0.f ? 1.0f / l : l != l ? l : 0.f;
+    const long out = (u.q0 + qt) * a.o_row + hq * a.o_head;
+    by_type(a.type, a.out, [&](auto* p) { store4(p + out + d4 * 4, o * inv, wide); });
+    if (a.lse && d4 == 0) a.lse[(u.q0 + qt) * (long)a.heads_q + hq] = (__log2f(l) + m - LIFT) * LN2;
   }
-  const float inv = l > 0.f ? 1.0f / l : l != l ? l : 0.f;
-  const long out = (u.q0 + qt) * a.o_row + hq * a.o_head;
-  store4(a.out, out + d4 * 4, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv, a.type, wide_stores(a));
-  if (a.lse && d4 == 0) a.lse[(u.q0 + qt) * (long)a.heads_q + hq] = (__log2f(l) + m - LIFT) * LN2;
 }
 
 // -------------------------------------------------------------------------------------------------------------------- host
-constexpr int NARROW_UNITS = 2048;      // parts of all kv heads that a read is divided into
-constexpr int NARROW_CHUNK = 16;        // fewest 32-token tiles worth a part
+#ifndef WU
+#define WU 512
+#endif
+#ifndef WC
+#define WC 16
+#endif
+#ifndef NL
+#define NL 64
+#endif
+constexpr int ROWS16 = 16;              // requests of at most this many rows per kv head take tiles of 16 rows
+constexpr int NARROW_ROWS = NL;         // up to this many the narrow kernel, beyond the wide one
+constexpr int NARROW_CHUNK = 8;         // fewest 32-token tiles worth a part
+constexpr int WIDE_UNITS = WU, WIDE_CHUNK = WC;
+constexpr int MERGE_Y = 32;             // rows of a tile that the merge gives waves of their own
 
+// parts of all kv heads that a read is divided into: as many as workgroups fit the chip at once
+int narrow_units(int dim) { return dim == 128 ? 512 : dim == 64 ? 1024 : 1536; }
+
+struct Launch {
+  Split sp;
+  int rows;                       // rows of a tile
+  long tiles, units, slots;       // per kv head: bounds of row tiles, units, partial results
+};
 struct Plan {
-  int G, ps, want;
-  long units, slots;      // per kv head: grid bound, partial results' bound
+  Launch narrow, wide;            // units 0: not used
 };
 
 bool valid_attn(const rmem_bank8_attn_args* a) {
@@ -506,35 +822,78 @@ bool valid_attn(const rmem_bank8_attn_args* a) {
   return (int64_t)a->rows * (a->heads_q / a->bank.heads) <= 0x7fffffff;
 }
 
-Plan make_plan(const rmem_bank8_attn_args* a) {
-  Plan p;
-  p.G = a->heads_q / a->bank.heads;
-  p.ps = log2_of(a->bank.page);
-  p.want = NARROW_UNITS / a->bank.heads;
-  if (p.want < 1) p.want = 1;
-  const long row_tiles = ((long)a->rows * p.G) / 32 + (a->reqs < a->rows ? a->reqs : a->rows);
+Launch make_launch(const rmem_bank8_attn_args* a, int rows, int units, int chunk_min, int lo, int hi) {
+  Launch l;
+  l.sp.G = a->heads_q / a->bank.heads;
+  l.sp.ps = log2_of(a->bank.page);
+  l.sp.want = units / a->bank.heads > 0 ? units / a->bank.heads : 1;
+  l.sp.chunk_min = chunk_min;
+  l.sp.lo = lo;
+  l.sp.hi = hi;
+  l.rows = rows;
+  l.tiles = (long)a->rows * l.sp.G / rows + (a->reqs < a->rows ? a->reqs : a->rows);
   // parts: at most total / chunk + one per row tile; of requests in several parts, at most twice total / chunk
-  p.units = p.want + row_tiles;
-  p.slots = 2L * p.want;
+  l.units = l.sp.want + l.tiles;
+  l.slots = 2L * l.sp.want;
+  return l;
+}
+
+Plan make_plan(const rmem_bank8_attn_args* a) {
+  const long most = (long)a->max_rows * (a->heads_q / a->bank.heads);
+  const int all = 0x7fffffff;
+  Plan p = {};
+  if (most <= NARROW_ROWS) p.narrow = make_launch(a, most <= ROWS16 ? 16 : 32, narrow_units(a->bank.dim), NARROW_CHUNK, 0, all);
+  else {
+    // one request: the wide kernel alone; several: the short ones among them in a launch of their own
+    p.wide = make_launch(a, WROWS, WIDE_UNITS, WIDE_CHUNK, a->reqs == 1 ? 0 : NARROW_ROWS + 1, all);
+    if (a->reqs > 1) p.narrow = make_launch(a, 32, narrow_units(a->bank.dim), NARROW_CHUNK, 0, NARROW_ROWS);
+  }
   return p;
 }
 
-long part_bytes(const rmem_bank8_attn_args* a, const Plan& p) {
-  return p.slots * a->bank.heads * 32 * (a->bank.dim + 2) * 4;
+long part_floats(const rmem_bank8_attn_args* a, const Launch& l) { return l.slots * a->bank.heads * l.rows * (a->bank.dim + 2); }
+
+template <int D, int CODE, int NS>
+void launch_attn(const rmem_bank8_attn_args& a, const Parts& parts, const Launch& l, hipStream_t s) {
+  const dim3 grid((unsigned)(l.units * a.bank.heads));
+  if (l.rows == 16) hipLaunchKernelGGL((attn_narrow<16, D, CODE, NS>), grid, dim3(256), 0, s, a, parts, l.sp);
+  else if (l.rows == 32) hipLaunchKernelGGL((attn_narrow<32, D, CODE, NS>), grid, dim3(256), 0, s, a, parts, l.sp);
+  else hipLaunchKernelGGL((attn_wide<D, CODE, NS>), grid, dim3(256), 0, s, a, parts, l.sp);
 }
 
-template <int D, int CODE>
-void launch_narrow(const rmem_bank8_attn_args& a, const Parts& parts, const Plan& p, hipStream_t s) {
-  const dim3 grid((unsigned)(p.units * a.bank.heads));
-  if (a.type == FP32) hipLaunchKernelGGL((attn_narrow<D, CODE, 2>), grid, dim3(256), 0, s, a, parts, p.G, p.ps, p.want, NARROW_CHUNK);
-  else hipLaunchKernelGGL((attn_narrow<D, CODE, 1>), grid, dim3(256), 0, s, a, parts, p.G, p.ps, p.want, NARROW_CHUNK);
+template <int D>
+int launch_dim(const rmem_bank8_attn_args& a, const Parts& parts, const Launch& l, hipStream_t s) {
+  const bool e4m3 = a.bank.code == E4M3, two = a.type == FP32;
+  if (e4m3) two ? launch_attn<D, E4M3, 2>(a, parts, l, s) : launch_attn<D, E4M3, 1>(a, parts, l, s);
+  else two ? launch_attn<D, INT8, 2>(a, parts, l, s) : launch_attn<D, INT8, 1>(a, parts, l, s);
+  RMEM_CHECK_LAUNCH();
+  // a request whose row of the table holds no more than the smallest part is never divided
+  if (((long)a.cols * a.bank.page + 31) / 32 > l.sp.chunk_min) {
+    const long tiles = l.tiles < l.sp.want ? l.tiles : l.sp.want;       // row tiles in at least two parts: at most `want`
+    const long rows = (long)a.max_rows * l.sp.G;
+    const dim3 grid((unsigned)(tiles * a.bank.heads), (unsigned)(rows >= 1 && rows < MERGE_Y ? rows : l.rows < MERGE_Y ? l.rows : MERGE_Y));
+    if (l.rows == 16) hipLaunchKernelGGL((attn_merge<16, D>), grid, dim3(64), 0, s, a, parts, l.sp);
+    else if (l.rows == 32) hipLaunchKernelGGL((attn_merge<32, D>), grid, dim3(64), 0, s, a, parts, l.sp);
+    else hipLaunchKernelGGL((attn_merge<WROWS, D>), grid, dim3(64), 0, s, a, parts, l.sp);
+    RMEM_CHECK_LAUNCH();
+  }
+  return RMEM_OK;
+}
+
+int launch_read(const rmem_bank8_attn_args& a, float* ws, const Launch& l, hipStream_t s) {
+  Parts parts;
+  parts.o = ws;
+  parts.ml = ws + l.slots * a.bank.heads * l.rows * a.bank.dim;
+  parts.slots = (int)l.slots;
+  return a.bank.dim == 32 ? launch_dim<32>(a, parts, l, s) : a.bank.dim == 64 ? launch_dim<64>(a, parts, l, s) : launch_dim<128>(a, parts, l, s);
 }
 
 }  // namespace
 
 extern "C" int64_t rmem_bank8_attn_workspace(const rmem_bank8_attn_args* a) {
   if (!valid_attn(a)) return -1;
-  return part_bytes(a, make_plan(a));
+  const Plan p = make_plan(a);
+  return 4 * ((p.narrow.units ? part_floats(a, p.narrow) : 0) + (p.wide.units ? part_floats(a, p.wide) : 0));
 }
 
 extern "C" int rmem_bank8_attn(const rmem_bank8_attn_args* a, void* stream) {
@@ -542,25 +901,14 @@ extern "C" int rmem_bank8_attn(const rmem_bank8_attn_args* a, void* stream) {
   if (a->rows == 0) return RMEM_OK;
   const Plan p = make_plan(a);
   if (!a->q || !a->out || !a->cu || !a->lens || !a->table || !a->workspace || ((uintptr_t)a->workspace % 16) ||
-      a->workspace_bytes < part_bytes(a, p) || p.units * a->bank.heads >= 1 << 24)
+      a->workspace_bytes < rmem_bank8_attn_workspace(a) || p.narrow.units * a->bank.heads >= 1 << 24 || p.wide.units * a->bank.heads >= 1 << 24)
     return RMEM_ERR_INVALID;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  Parts parts;
-  parts.o = static_cast<float*>(a->workspace);
-  parts.ml = parts.o + p.slots * a->bank.heads * 32 * a->bank.dim;
-  parts.slots = (int)p.slots;
-  const bool e4m3 = a->bank.code == E4M3;
-  switch (a->bank.dim) {
-    case 32: e4m3 ? launch_narrow<32, E4M3>(*a, parts, p, s) : launch_narrow<32, INT8>(*a, parts, p, s); break;
-    case 64: e4m3 ? launch_narrow<64, E4M3>(*a, parts, p, s) : launch_narrow<64, INT8>(*a, parts, p, s); break;
-    default: e4m3 ? launch_narrow<128, E4M3>(*a, parts, p, s) : launch_narrow<128, INT8>(*a, parts, p, s); break;
+  float* ws = static_cast<float*>(a->workspace);
+  if (p.wide.units) {
+    const int rc = launch_read(*a, ws, p.wide, s);
+    if (rc != RMEM_OK) return rc;
+    ws += part_floats(a, p.wide);
   }
-  RMEM_CHECK_LAUNCH();
-  // a request whose row of the table holds no more than the smallest part is never divided
-  if (((long)a->cols * a->bank.page + 31) / 32 > NARROW_CHUNK) {
-    const long tiles = p.slots / 2;       // row tiles in at least two parts
-    hipLaunchKernelGGL((attn_merge<32>), dim3((unsigned)(tiles * a->bank.heads), 32), dim3(256), 0, s, *a, parts, p.G, p.want, NARROW_CHUNK);
-    RMEM_CHECK_LAUNCH();
-  }
-  return RMEM_OK;
+  return p.narrow.units ? launch_read(*a, ws, p.narrow, s) : RMEM_OK;
 }
