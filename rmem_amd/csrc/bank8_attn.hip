@@ -9,10 +9,11 @@
 // denominator takes each tile's sum of weights times 1 / vs.  No dequantised value exists anywhere.
 // Queries enter as fp16 times a power of two per row that puts the row's largest element at 2^14: fp16 and bf16 rows are exact
 // down to 2^-38 of that element; fp32 rows keep 22 bits in two planes (NS = 2: two products against the same codes).
-// Weights are 2^10 times their usual size (the maximum is 2^10, not 1), which leaves 24 instead of 14 binades of normal fp16
-// numbers below the maximum; fp32 calls keep them in two planes.  Sums are fp32, of the unrounded weights.
+// Weights are 2^10 times their usual size (2^10 at the row's reference, not 1), which leaves 24 instead of 14 binades of normal
+// fp16 numbers below it; fp32 calls keep them in two planes.  Sums are fp32, of the unrounded weights.
 #include "bank8.h"
 
+#include <algorithm>
 #include <type_traits>
 
 using namespace bank8;
@@ -22,9 +23,10 @@ using namespace bank8;
 namespace {
 
 constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
-constexpr float LIFT = 10.f;             // log2 of the largest weight
+constexpr float LIFT = 10.f;             // log2 of a weight at the row's reference
+constexpr float SLACK = 5.f;             // how far the maximum may get ahead of it
 constexpr float LOWEST = -3.0e38f;       // running maximum of a row that has seen nothing
-constexpr float VS_MIN = 1.262177448e-29f;   // 2^-96: 1 / vs times 2^10 times 2^20 tokens stays finite
+constexpr float VS_MIN = 3.23117427e-27f;    // 2^-88: 1 / vs times 2^15 times 2^24 tokens stays finite
 
 // ---------------------------------------------------------------------------------------------------- division into units
 // A unit of work is (request, tile of ROWS rows, one of ns equal parts of the tokens that the tile sees) for one kv head.  Every
@@ -34,7 +36,7 @@ constexpr float VS_MIN = 1.262177448e-29f;   // 2^-96: 1 / vs times 2^10 times 2
 struct Unit {
   int r, rt, part, ns;    // request, row tile, part of ns
   int q0, n, len;         // first row, rows, tokens
-  int slot;               // index of the partial result of part 0 (ns > 1)
+  int slot, ord;          // of a row tile in several parts: index of part 0's partial result, index among such tiles
 };
 
 struct Req {
@@ -74,52 +76,73 @@ __device__ __forceinline__ long wave_sum_long(long v) {
   return v;
 }
 
-// by_parts: index counts (request, row tile, part); otherwise (request, row tile) of requests in more than one part (the merge).
+// tiles of a part
 template <int ROWS>
-__device__ bool find_unit(const rmem_bank8_attn_args& a, const Split& sp, long index, bool by_parts, Unit& u) {
+__device__ __forceinline__ int chunk_of(const rmem_bank8_attn_args& a, const Split& sp, const Req& first) {
   const int lane = threadIdx.x & 63;
-  Req x = request<ROWS>(a, lane, sp);
-  long total = (long)x.rt * x.tiles;
+  long total = (long)first.rt * first.tiles;
   for (int b = 64; b < a.reqs; b += 64) {
     const Req y = request<ROWS>(a, b + lane, sp);
     total += (long)y.rt * y.tiles;
   }
-  total = wave_sum_long(total);
-  total = (total + sp.want - 1) / sp.want;
-  const int chunk = total < sp.chunk_min ? sp.chunk_min : total > 0x3fffffff ? 0x3fffffff : (int)total;
-  long seen = 0, slots = 0;
+  total = (wave_sum_long(total) + sp.want - 1) / sp.want;
+  return total < sp.chunk_min ? sp.chunk_min : total > 0x3fffffff ? 0x3fffffff : (int)total;
+}
+
+template <int ROWS>
+__device__ bool find_unit(const rmem_bank8_attn_args& a, const Split& sp, long index, Unit& u) {
+  const int lane = threadIdx.x & 63;
+  Req x = request<ROWS>(a, lane, sp);
+  const int chunk = chunk_of<ROWS>(a, sp, x);
+  long seen = 0, slots = 0, ords = 0;
   for (int b = 0; b < a.reqs; b += 64) {
     if (b) x = request<ROWS>(a, b + lane, sp);
     const int ns = x.tiles > chunk ? (x.tiles + chunk - 1) / chunk : 1;
-    const int split = ns > 1 ? x.rt * ns : 0;
-    int cnt = by_parts ? x.rt * ns : ns > 1 ? x.rt : 0;
-    int c = cnt, s = split;
+    const int cnt = x.rt * ns, split = ns > 1 ? cnt : 0, ord = ns > 1 ? x.rt : 0;
+    int c = cnt, s = split, o = ord;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int cu = __shfl_up(c, o), su = __shfl_up(s, o);
-      if (lane >= o) {
+    for (int d = 1; d < 64; d <<= 1) {
+      const int cu = __shfl_up(c, d), su = __shfl_up(s, d), ou = __shfl_up(o, d);
+      if (lane >= d) {
         c += cu;
         s += su;
+        o += ou;
       }
     }
     const unsigned long long hit = __ballot(index < seen + c);
     if (hit) {
       const int l = __builtin_ctzll(hit);
       u.ns = __builtin_amdgcn_readlane(ns, l);
-      int k = (int)(index - seen) - (__builtin_amdgcn_readlane(c, l) - __builtin_amdgcn_readlane(cnt, l));
+      const int k = (int)(index - seen) - (__builtin_amdgcn_readlane(c, l) - __builtin_amdgcn_readlane(cnt, l));
       u.r = b + l;
-      u.rt = by_parts ? k / u.ns : k;
-      u.part = by_parts ? k - u.rt * u.ns : 0;
+      u.rt = __builtin_amdgcn_readlane(x.rt, l) - 1 - k / u.ns;      // the last row tile first: under a causal mask it sees most
+      u.part = k % u.ns;
       u.q0 = __builtin_amdgcn_readlane(x.q0, l);
       u.n = __builtin_amdgcn_readlane(x.n, l);
       u.len = __builtin_amdgcn_readlane(x.len, l);
       u.slot = (int)slots + __builtin_amdgcn_readlane(s, l) - __builtin_amdgcn_readlane(split, l) + u.rt * u.ns;
+      u.ord = (int)ords + __builtin_amdgcn_readlane(o, l) - __builtin_amdgcn_readlane(ord, l) + u.rt;
       return true;
     }
     seen += __builtin_amdgcn_readlane(c, 63);
     slots += __builtin_amdgcn_readlane(s, 63);
+    ords += __builtin_amdgcn_readlane(o, 63);
   }
   return false;
+}
+
+// row tiles in several parts
+template <int ROWS>
+__device__ __forceinline__ long count_split(const rmem_bank8_attn_args& a, const Split& sp) {
+  const int lane = threadIdx.x & 63;
+  Req x = request<ROWS>(a, lane, sp);
+  const int chunk = chunk_of<ROWS>(a, sp, x);
+  long n = 0;
+  for (int b = 0; b < a.reqs; b += 64) {
+    if (b) x = request<ROWS>(a, b + lane, sp);
+    if (x.tiles > chunk) n += x.rt;
+  }
+  return wave_sum_long(n);
 }
 
 // ---------------------------------------------------------------------------------------------------------- one token tile
@@ -275,84 +298,97 @@ struct Acc {
   }
 };
 
-// tokens tok0 .. tok0 + 31 against this lane's row, which sees tokens < lim; kf(step[, chain]), vf(dim tile[, step]) give fragments
-template <int R, int D, int NS, class KF, class VF>
-__device__ __forceinline__ void tile(Acc<R, D>& c, const Query<R, D, NS>& q, int tok0, int lim, float ks, float lvs, float ivs, int g, bool masked,
-                                     KF kf, VF vf) {
-  constexpr int N = R / 2;                  // tokens per lane
-  float s[N];
-  if constexpr (R == 32) {
-    f32x16_t x;
+// T tiles of 32 tokens from tok0 on, against this lane's row, which sees the tokens below lim[t] of tile t; kf(t, step, chain) and
+// vf(t, dim tile, step) give fragments.  One maximum and one look at the accumulators for all T: a row's reference m follows the
+// maximum only when that gets SLACK ahead, because weights up to 2^(LIFT + SLACK) fit into fp16 -- after the first few tiles the
+// accumulators are hardly ever scaled again.
+template <int T, int R, int D, int NS, class KF, class VF>
+__device__ __forceinline__ void attend_tiles(Acc<R, D>& c, const Query<R, D, NS>& q, int tok0, const int (&lim)[T], const float (&ks)[T],
+                                      const float (&lvs)[T], const float (&ivs)[T], int g, bool masked, KF kf, VF vf) {
+  constexpr int N = R / 2;                  // tokens per lane and tile
+  float s[T][N];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) x[r] = 0.f;
+  for (int i = 0; i < T; ++i) {
+    if constexpr (R == 32) {
+      f32x16_t x;
 #pragma unroll
-    for (int t = 0; t < D / 16; ++t) {
-      const frag8_t k = kf(t, 0);
-      if constexpr (NS == 2) x = RMEM_MFMA(k, q.f[NS - 1][t], x);
-      x = RMEM_MFMA(k, q.f[0][t], x);
-    }
+      for (int r = 0; r < 16; ++r) x[r] = 0.f;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = x[r];
-  } else {
-    f32x4_t x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-    for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const frag8_t f = kf(t, k);
-        if constexpr (NS == 2) x[k] = MFMA16(f, q.f[NS - 1][t], x[k]);
-        x[k] = MFMA16(f, q.f[0][t], x[k]);
+      for (int t = 0; t < D / 16; ++t) {
+        const frag8_t k = kf(i, t, 0);
+        if constexpr (NS == 2) x = RMEM_MFMA(k, q.f[NS - 1][t], x);
+        x = RMEM_MFMA(k, q.f[0][t], x);
       }
 #pragma unroll
-    for (int r = 0; r < 8; ++r) s[r] = x[r >> 2][r & 3];
-  }
-  const float mul = q.mul * ks;
-  float top;
-  const int left = lim - tok0 - (R == 32 ? 4 * g : 16 * (g & 1) + 4 * (g >> 1));   // register r holds token (r & 3) + 8 (r >> 2) of these
-  if (!masked) {
-    top = s[0];
+      for (int r = 0; r < 16; ++r) s[i][r] = x[r];
+    } else {
+      f32x4_t x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-    for (int r = 1; r < N; ++r) top = fmaxf(top, s[r]);
-    top = fmaf(top, mul, lvs);
-  } else {
-    top = LOWEST;
+      for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-    for (int r = 0; r < N; ++r) top = fmaxf(top, (r & 3) + 8 * (r >> 2) < left ? fmaf(s[r], mul, lvs) : LOWEST);
-  }
-  const float m = fmaxf(c.m, row_max<R>(top));
-  const float add = lvs - m + LIFT;
-  float w[N], sum = 0.f;
+        for (int k = 0; k < 2; ++k) {
+          const frag8_t f = kf(i, t, k);
+          if constexpr (NS == 2) x[k] = MFMA16(f, q.f[NS - 1][t], x[k]);
+          x[k] = MFMA16(f, q.f[0][t], x[k]);
+        }
 #pragma unroll
-  for (int r = 0; r < N; ++r) {
-    w[r] = __builtin_amdgcn_exp2f(fmaf(s[r], mul, add));
-    if (masked) w[r] = (r & 3) + 8 * (r >> 2) < left ? w[r] : 0.f;
-    sum += w[r];
+      for (int r = 0; r < 8; ++r) s[i][r] = x[r >> 2][r & 3];
+    }
   }
-  sum = row_sum<R>(sum) * ivs;
-  if (__any(m != c.m)) {
+  if (masked) {
+    // register r holds token (r & 3) + 8 (r >> 2) of these; the pin keeps this a branch (as selects it costs every tile)
+    int at = R == 32 ? 4 * g : 16 * (g & 1) + 4 * (g >> 1);
+    asm volatile("" : "+v"(at));
+#pragma unroll
+    for (int i = 0; i < T; ++i)
+#pragma unroll
+      for (int r = 0; r < N; ++r) s[i][r] = (r & 3) + 8 * (r >> 2) < lim[i] - tok0 - 32 * i - at ? s[i][r] : -INFINITY;
+  }
+  float mul[T], top = LOWEST;
+#pragma unroll
+  for (int i = 0; i < T; ++i) {
+    mul[i] = fmaxf(q.mul * ks[i], 1.4e-45f);      // positive: times -infinity it stays that
+    float x = s[i][0];
+#pragma unroll
+    for (int r = 1; r < N; ++r) x = fmaxf(x, s[i][r]);
+    top = fmaxf(top, fmaf(x, mul[i], lvs[i]));
+  }
+  top = row_max<R>(top);
+  if (__any(top > c.m + SLACK)) {
+    const float m = top > c.m + SLACK ? top : c.m;
     const float alpha = __builtin_amdgcn_exp2f(c.m - m);
     c.l *= alpha;
     c.mul(alpha);
     c.m = m;
   }
-  c.l += sum;
 #pragma unroll
-  for (int st = 0; st < N / 8; ++st) {
-    frag8_t p, pl;
+  for (int i = 0; i < T; ++i) {
+    const float add = lvs[i] - c.m + LIFT;
+    float sum[2] = {0.f, 0.f};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      p[e] = (_Float16)w[8 * st + e];
-      if constexpr (NS == 2) pl[e] = (_Float16)(w[8 * st + e] - (float)p[e]);
+    for (int r = 0; r < N; ++r) {
+      s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], mul[i], add));
+      sum[r & 1] += s[i][r];
     }
+    c.l = fmaf(sum[0] + sum[1], ivs[i], c.l);     // this lane's tokens; joined with its row's other lanes at the end
 #pragma unroll
-    for (int d = 0; d < D / R; ++d) {
-      const frag8_t v = vf(d, st);
-      if constexpr (R == 32) {
-        if constexpr (NS == 2) c.o[d] = RMEM_MFMA(v, pl, c.o[d]);
-        c.o[d] = RMEM_MFMA(v, p, c.o[d]);
-      } else {
-        if constexpr (NS == 2) c.o[d] = MFMA16(v, pl, c.o[d]);
-        c.o[d] = MFMA16(v, p, c.o[d]);
+    for (int st = 0; st < N / 8; ++st) {
+      frag8_t p, pl;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = (_Float16)s[i][8 * st + e];
+        if constexpr (NS == 2) pl[e] = (_Float16)(s[i][8 * st + e] - (float)p[e]);
+      }
+#pragma unroll
+      for (int d = 0; d < D / R; ++d) {
+        const frag8_t v = vf(i, d, st);
+        if constexpr (R == 32) {
+          if constexpr (NS == 2) c.o[d] = RMEM_MFMA(v, pl, c.o[d]);
+          c.o[d] = RMEM_MFMA(v, p, c.o[d]);
+        } else {
+          if constexpr (NS == 2) c.o[d] = MFMA16(v, pl, c.o[d]);
+          c.o[d] = MFMA16(v, p, c.o[d]);
+        }
       }
     }
   }
@@ -400,15 +436,26 @@ __device__ __forceinline__ void write_row(const rmem_bank8_attn_args& a, const A
   if (a.lse && g == 0) a.lse[row * a.heads_q + hq] = (__log2f(c.l) + c.m - LIFT) * LN2;
 }
 
-// partial results of split units: [slot][kv head][ROWS][D] fp32, then [slot][kv head][ROWS][2] (maximum, sum)
+// partial results of split units: [slot][kv head][ROWS][D] fp32, [slot][kv head][ROWS][2] (reference, sum), and for each row tile
+// in several parts what the merge needs to know of it
+struct Split_tile {
+  int q0, n, rt, ns, slot, pad[3];
+};
 struct Parts {
   float* o;
   float* ml;
-  int slots;              // units that fit
+  Split_tile* tiles;
+  int slots, ords;        // units and tiles that fit
 };
 
 template <int ROWS, int R, int D>
-__device__ __forceinline__ void write_part(const Parts& w, const Acc<R, D>& c, int slot, int h, int heads, int j, int g) {
+__device__ __forceinline__ void write_part(const Parts& w, const Acc<R, D>& c, const Unit& u, int h, int heads, int j, int g) {
+  const int slot = u.slot + u.part;
+  if (slot >= w.slots) return;
+  if (h == 0 && u.part == 0 && j == 0 && g == 0 && u.ord < w.ords) {
+    const Split_tile t = {u.q0, u.n, u.rt, u.ns, u.slot, {0, 0, 0}};
+    w.tiles[u.ord] = t;
+  }
   const long row = ((long)slot * heads + h) * ROWS + j;
 #pragma unroll
   for (int i = 0; i < Acc<R, D>::QUADS; ++i) *reinterpret_cast<f32x4_t*>(w.o + row * D + Acc<R, D>::STRIDE * i + 4 * g) = c.quad(i);
@@ -512,7 +559,7 @@ __global__ __launch_bounds__(256, 2) void attn_narrow(rmem_bank8_attn_args a, Pa
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);       // uniform: tile counts and page addresses stay scalar
   const int heads = a.bank.heads, h = blockIdx.x % heads;
   Unit u;
-  if (!find_unit<R>(a, sp, blockIdx.x / heads, true, u)) return;
+  if (!find_unit<R>(a, sp, blockIdx.x / heads, u)) return;
   const int row = u.rt * R + j, qt = row / G, hq = h * G + row % G;
   const bool on = qt < u.n;
   const int lim = !on ? 0 : a.causal ? min(u.len, u.len - u.n + qt + 1) : u.len;     // may be <= 0
@@ -557,8 +604,10 @@ __global__ __launch_bounds__(256, 2) void attn_narrow(rmem_bank8_attn_args a, Pa
       const bool absent = __builtin_amdgcn_readlane(pid, i) < 0;
       const int end = absent ? tok0 : u.len;
       if (CODE == E4M3 && tok0 + 32 > end) x.cut(end - tok0, g);
-      tile<R, D, NS>(c, q, tok0, min(lim, end), readlane(ks, i), readlane(lvs, i), readlane(ivs, i), g, tok0 + 32 > min(see.all, end),
-                     [&](int t, int k) { return x.template kf<CODE>(t, k); }, [&](int d, int st) { return x.template vf<CODE>(d, st); });
+      const int lims[1] = {min(lim, end)};
+      const float k1[1] = {readlane(ks, i)}, l1[1] = {readlane(lvs, i)}, i1[1] = {readlane(ivs, i)};
+      attend_tiles<1, R, D, NS>(c, q, tok0, lims, k1, l1, i1, g, tok0 + 32 > min(see.all, end),
+                         [&](int, int t, int k) { return x.template kf<CODE>(t, k); }, [&](int, int d, int st) { return x.template vf<CODE>(d, st); });
     };
     // The loads are unconditional (the last tile again where there is no next one): with a way around them the compiler would have
     // to wait for all that may be in flight before it touches the present tile.
@@ -573,7 +622,8 @@ __global__ __launch_bounds__(256, 2) void attn_narrow(rmem_bank8_attn_args a, Pa
     }
   }
 
-  // join the four waves
+  // join the lanes of a row, then the four waves
+  c.l = row_sum<R>(c.l);
   s_m[wave][lane] = c.m;
   s_l[wave][lane] = c.l;
   __syncthreads();
@@ -602,7 +652,7 @@ __global__ __launch_bounds__(256, 2) void attn_narrow(rmem_bank8_attn_args a, Pa
   get(0);
   if (!on) return;
   if (u.ns == 1) write_row<R, D>(a, c, hq, u.q0 + qt, g);
-  else if (u.slot + u.part < parts.slots) write_part<R, R, D>(parts, c, u.slot + u.part, h, heads, j, g);
+  else write_part<R, R, D>(parts, c, u, h, heads, j, g);
 }
 
 // ------------------------------------------------------------------------------------------------------ many rows per head
@@ -615,7 +665,7 @@ __global__ __launch_bounds__(256, 2) void attn_narrow(rmem_bank8_attn_args a, Pa
 constexpr int WROWS = 128;
 
 template <int D, int CODE, int NS>
-__global__ __launch_bounds__(256, 2) void attn_wide(rmem_bank8_attn_args a, Parts parts, Split sp) {
+__global__ __launch_bounds__(256, NS == 2 && D == 128 ? 1 : 2) void attn_wide(rmem_bank8_attn_args a, Parts parts, Split sp) {
   constexpr int R = 32, CH = D / 32;             // 16-byte chunks per thread and stage: 8 D / 256
   constexpr int HALF = 64 * D / 8;               // fragments (16 bytes) of a stage's keys; as many of its values
   __shared__ __attribute__((aligned(16))) u32x4_t s_kv[2][2 * HALF];
@@ -624,7 +674,7 @@ __global__ __launch_bounds__(256, 2) void attn_wide(rmem_bank8_attn_args a, Part
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int heads = a.bank.heads, h = blockIdx.x % heads;
   Unit u;
-  if (!find_unit<WROWS>(a, sp, blockIdx.x / heads, true, u)) return;
+  if (!find_unit<WROWS>(a, sp, blockIdx.x / heads, u)) return;
   const int row0 = u.rt * WROWS + wave * R, row = row0 + j, qt = row / G, hq = h * G + row % G;
   const bool on = qt < u.n;
   const int lim = !on ? 0 : a.causal ? min(u.len, u.len - u.n + qt + 1) : u.len;
@@ -654,7 +704,10 @@ __global__ __launch_bounds__(256, 2) void attn_wide(rmem_bank8_attn_args a, Part
   int page0 = -1, page1 = -1;                    // pages of the two tiles in `raw`
   int load_pid = -1;                             // pages of the 64 tiles around them
   auto load = [&](int st) __attribute__((always_inline)) {
-    if ((st & 31) == 0) load_pid = pages_of(st >> 5);
+    if ((st & 31) == 0) {
+      load_pid = pages_of(st >> 5);
+      asm volatile("" : "+v"(load_pid));         // waited for here: behind the branch every stage would wait for all loads in flight
+    }
     const int i = (2 * st) & 63, ta = t0 + 2 * st;
     page0 = __builtin_amdgcn_readlane(load_pid, i);
     page1 = __builtin_amdgcn_readlane(load_pid, i + 1);
@@ -712,34 +765,42 @@ __global__ __launch_bounds__(256, 2) void attn_wide(rmem_bank8_attn_args a, Part
     if ((st & 31) == 0) {
       pid = pages_of(st >> 5);
       float vs = 1.f;
+      ks = 0.f;
       if (pid >= 0) {
         ks = a.bank.k_scale[(long)pid * heads + h];
         vs = fmaxf(a.bank.v_scale[(long)pid * heads + h], VS_MIN);
       }
       lvs = __log2f(vs);
       ivs = 1.0f / vs;
+      asm volatile("" : "+v"(pid), "+v"(ks));    // as above
     }
     __syncthreads();                             // stage st is in its buffer, and every wave is done with the other one
     if (st + 1 < stages) put(st + 1, s_kv[(st + 1) & 1]);
     if (st + 2 < stages) load(st + 2);
     const u32x4_t* kv = s_kv[st & 1];
-#pragma unroll 1
-    for (int sub = 0; sub < 2; ++sub) {
-      const int t = t0 + 2 * st + sub, i = (2 * st + sub) & 63, tok0 = t * 32;
-      if (t >= t1 || tok0 >= see.sees || __builtin_amdgcn_readlane(pid, i) < 0) continue;
-      tile<R, D, NS>(c, q, tok0, lim, readlane(ks, i), readlane(lvs, i), readlane(ivs, i), g, tok0 + 32 > min(see.all, u.len),
-                     [&](int k, int) { return __builtin_bit_cast(frag8_t, kv[(sub * (D / 16) + k) * 64 + lane]); },
-                     [&](int d, int k) { return __builtin_bit_cast(frag8_t, kv[HALF + ((sub * (D / 32) + d) * 2 + k) * 64 + lane]); });
-    }
+    const int t = t0 + 2 * st, i = (2 * st) & 63, tok0 = t * 32;
+    if (tok0 >= see.sees) continue;
+    const bool gone0 = __builtin_amdgcn_readlane(pid, i) < 0, gone1 = __builtin_amdgcn_readlane(pid, i + 1) < 0;   // (-1 from t1 on)
+    const int lims[2] = {gone0 ? tok0 : lim, gone1 ? tok0 + 32 : lim};
+    const float k2[2] = {readlane(ks, i), readlane(ks, i + 1)}, l2[2] = {readlane(lvs, i), readlane(lvs, i + 1)},
+                i2[2] = {readlane(ivs, i), readlane(ivs, i + 1)};
+    attend_tiles<2, R, D, NS>(c, q, tok0, lims, k2, l2, i2, g, gone0 || gone1 || tok0 + 64 > min(see.all, u.len),
+                       [&](int sub, int k, int) { return __builtin_bit_cast(frag8_t, kv[(sub * (D / 16) + k) * 64 + lane]); },
+                       [&](int sub, int d, int k) { return __builtin_bit_cast(frag8_t, kv[HALF + ((sub * (D / 32) + d) * 2 + k) * 64 + lane]); });
   }
+  c.l = row_sum<R>(c.l);
   if (!on) return;
   if (u.ns == 1) write_row<R, D>(a, c, hq, u.q0 + qt, g);
-  else if (u.slot + u.part < parts.slots) write_part<WROWS, R, D>(parts, c, u.slot + u.part, h, heads, wave * R + j, g);
+  else write_part<WROWS, R, D>(parts, c, u, h, heads, wave * R + j, g);
 }
 
 // ------------------------------------------------------------------------------------------------------------------- merge
-// One wave per (row tile of a split request, kv head, row): D / 4 lanes per part, the row's parts in order over the 256 / D groups
-// of lanes.  Waves of their own so that one round of them fills the chip: most of a call's grid finds nothing to do.
+// One workgroup per (row tile in several parts, kv head, BLOCK rows of the tile), a fixed number of workgroups that step through
+// them: a grid for the most there could be costs more than the work (most calls have few or none).  Few parts: one thread per
+// four dims of a row, which walks them.  Many: a wave per row, the parts over its 256 / D groups of lanes.
+constexpr int merge_block(int rows) { return rows == 16 ? 4 : rows == 32 ? 8 : 16; }
+constexpr int FEW_PARTS = 8;
+
 template <int D>
 __device__ __forceinline__ float over_groups(float x) {       // sum over the lanes that hold the same dims
   x += xor_lane<32>(x);
@@ -747,63 +808,93 @@ __device__ __forceinline__ float over_groups(float x) {       // sum over the la
   if constexpr (D <= 32) x += xor_lane<8>(x);
   return x;
 }
+
 template <int ROWS, int D>
-__global__ __launch_bounds__(64) void attn_merge(rmem_bank8_attn_args a, Parts parts, Split sp) {
-  const int heads = a.bank.heads, lane = threadIdx.x, G = sp.G;
-  const int h = blockIdx.x % heads;
-  Unit u;
-  if (!find_unit<ROWS>(a, sp, blockIdx.x / heads, false, u)) return;
-  if (u.slot + u.ns > parts.slots) return;
-  constexpr int WIDTH = D / 4, GROUPS = 64 / WIDTH;
-  const int g = lane / WIDTH, d4 = lane % WIDTH;
+__global__ __launch_bounds__(256) void attn_merge(rmem_bank8_attn_args a, Parts parts, Split sp) {
+  constexpr int WIDTH = D / 4, GROUPS = 64 / WIDTH, BLOCK = merge_block(ROWS), BLOCKS = ROWS / BLOCK;
+  const int heads = a.bank.heads, lane = threadIdx.x & 63, G = sp.G;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool wide = wide_stores(a);
-  for (int j = blockIdx.y; j < ROWS; j += gridDim.y) {
-    const int row = u.rt * ROWS + j, qt = row / G, hq = h * G + row % G;
-    if (qt >= u.n) break;
-    const long first = ((long)u.slot * heads + h) * ROWS + j, step = (long)heads * ROWS;
-    float m = LOWEST;
-    for (int p = lane; p < u.ns; p += 64) m = fmaxf(m, parts.ml[(first + p * step) * 2]);
-    m = wave_max_xor(m);
-    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-#pragma unroll 8
-    for (int p = g; p < u.ns; p += GROUPS) {
-      const long at = first + p * step;
-      const float f = __builtin_amdgcn_exp2f(parts.ml[at * 2] - m);
-      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(parts.o + at * D + d4 * 4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
-      l = fmaf(parts.ml[at * 2 + 1], f, l);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = over_groups<D>(o[e]);
-    l = over_groups<D>(l);
-    if (g) continue;
+  const long tiles = count_split<ROWS>(a, sp), items = (tiles < parts.ords ? tiles : parts.ords) * heads * BLOCKS;
+  auto finish = [&](const Split_tile& t, int h, int j, int d4, f32x4_t o, float m, float l, bool mine) __attribute__((always_inline)) {
+    const int row = t.rt * ROWS + j, hq = h * G + row % G;
+    const long at = t.q0 + row / G;
     const float inv = l > 0.f ? 1.0f / l : l != l ? l : 0.f;
-    const long out = (u.q0 + qt) * a.o_row + hq * a.o_head;
-    by_type(a.type, a.out, [&](auto* p) { store4(p + out + d4 * 4, o * inv, wide); });
-    if (a.lse && d4 == 0) a.lse[(u.q0 + qt) * (long)a.heads_q + hq] = (__log2f(l) + m - LIFT) * LN2;
+    if (mine) {
+      by_type(a.type, a.out, [&](auto* p) { store4(p + at * a.o_row + hq * a.o_head + d4 * 4, o * inv, wide); });
+      if (a.lse && d4 == 0) a.lse[at * a.heads_q + hq] = (__log2f(l) + m - LIFT) * LN2;
+    }
+  };
+  for (long item = blockIdx.x; item < items; item += gridDim.x) {
+    const long th = item / BLOCKS;
+    const int h = (int)(th % heads), end = (int)(item % BLOCKS + 1) * BLOCK;
+    const Split_tile t = parts.tiles[th / heads];
+    if (t.slot + t.ns > parts.slots) continue;
+    const int rows = min(end, t.n * G - t.rt * ROWS);        // of the tile that exist (n * G < 2^31: checked on the host)
+    const long step = (long)heads * ROWS;
+    if (t.ns <= FEW_PARTS) {
+      const int d4 = threadIdx.x % WIDTH;
+      for (int j = end - BLOCK + threadIdx.x / WIDTH; j < rows; j += 256 / WIDTH) {
+        const long first = ((long)t.slot * heads + h) * ROWS + j;
+        float pm[FEW_PARTS], pl[FEW_PARTS], m = LOWEST, l = 0.f;
+        f32x4_t x[FEW_PARTS], o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int p = 0; p < FEW_PARTS; ++p) {
+          const long at = first + min(p, t.ns - 1) * step;
+          pm[p] = parts.ml[at * 2];
+          pl[p] = parts.ml[at * 2 + 1];
+          x[p] = *reinterpret_cast<const f32x4_t*>(parts.o + at * D + d4 * 4);
+        }
+#pragma unroll
+        for (int p = 0; p < FEW_PARTS; ++p) m = fmaxf(m, pm[p]);
+#pragma unroll
+        for (int p = 0; p < FEW_PARTS; ++p) {
+          const float f = p < t.ns ? __builtin_amdgcn_exp2f(pm[p] - m) : 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = p < t.ns ? fmaf(x[p][e], f, o[e]) : o[e];
+          l = p < t.ns ? fmaf(pl[p], f, l) : l;
+        }
+        finish(t, h, j, d4, o, m, l, true);
+      }
+    } else {
+      const int g = lane / WIDTH, d4 = lane % WIDTH;
+      for (int j = end - BLOCK + wave; j < rows; j += 4) {
+        const long first = ((long)t.slot * heads + h) * ROWS + j;
+        float m = LOWEST;
+        for (int p = lane; p < t.ns; p += 64) m = fmaxf(m, parts.ml[(first + p * step) * 2]);
+        m = wave_max_xor(m);
+        f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+        float l = 0.f;
+#pragma unroll 8
+        for (int p = g; p < t.ns; p += GROUPS) {
+          const long at = first + p * step;
+          const float f = __builtin_amdgcn_exp2f(parts.ml[at * 2] - m);
+          const f32x4_t x = *reinterpret_cast<const f32x4_t*>(parts.o + at * D + d4 * 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
+          l = fmaf(parts.ml[at * 2 + 1], f, l);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = over_groups<D>(o[e]);
+        l = over_groups<D>(l);
+        finish(t, h, j, d4, o, m, l, g == 0);
+      }
+    }
   }
 }
 
 // -------------------------------------------------------------------------------------------------------------------- host
-#ifndef WU
-#define WU 512
-#endif
-#ifndef WC
-#define WC 16
-#endif
 #ifndef NL
-#define NL 64
+#define NL 256
 #endif
 constexpr int ROWS16 = 16;              // requests of at most this many rows per kv head take tiles of 16 rows
 constexpr int NARROW_ROWS = NL;         // up to this many the narrow kernel, beyond the wide one
 constexpr int NARROW_CHUNK = 8;         // fewest 32-token tiles worth a part
-constexpr int WIDE_UNITS = WU, WIDE_CHUNK = WC;
-constexpr int MERGE_Y = 32;             // rows of a tile that the merge gives waves of their own
+constexpr int WIDE_CHUNK = 16;
 
 // parts of all kv heads that a read is divided into: as many as workgroups fit the chip at once
 int narrow_units(int dim) { return dim == 128 ? 512 : dim == 64 ? 1024 : 1536; }
+int wide_units(int dim) { return dim == 128 ? 512 : 2048; }
 
 struct Launch {
   Split sp;
@@ -831,7 +922,9 @@ Launch make_launch(const rmem_bank8_attn_args* a, int rows, int units, int chunk
   l.sp.lo = lo;
   l.sp.hi = hi;
   l.rows = rows;
-  l.tiles = (long)a->rows * l.sp.G / rows + (a->reqs < a->rows ? a->reqs : a->rows);
+  const long reqs = std::min(a->reqs, a->rows);            // with rows
+  l.tiles = (long)a->rows * l.sp.G / rows + reqs;
+  l.tiles = std::min(l.tiles, reqs * (((long)hi + rows - 1) / rows));
   // parts: at most total / chunk + one per row tile; of requests in several parts, at most twice total / chunk
   l.units = l.sp.want + l.tiles;
   l.slots = 2L * l.sp.want;
@@ -845,13 +938,16 @@ Plan make_plan(const rmem_bank8_attn_args* a) {
   if (most <= NARROW_ROWS) p.narrow = make_launch(a, most <= ROWS16 ? 16 : 32, narrow_units(a->bank.dim), NARROW_CHUNK, 0, all);
   else {
     // one request: the wide kernel alone; several: the short ones among them in a launch of their own
-    p.wide = make_launch(a, WROWS, WIDE_UNITS, WIDE_CHUNK, a->reqs == 1 ? 0 : NARROW_ROWS + 1, all);
+    p.wide = make_launch(a, WROWS, wide_units(a->bank.dim), WIDE_CHUNK, a->reqs == 1 ? 0 : NARROW_ROWS + 1, all);
     if (a->reqs > 1) p.narrow = make_launch(a, 32, narrow_units(a->bank.dim), NARROW_CHUNK, 0, NARROW_ROWS);
   }
   return p;
 }
 
-long part_floats(const rmem_bank8_attn_args* a, const Launch& l) { return l.slots * a->bank.heads * l.rows * (a->bank.dim + 2); }
+// floats of a launch's workspace: partial results, references and sums, tiles in several parts (at most `want`: two parts each)
+long part_floats(const rmem_bank8_attn_args* a, const Launch& l) {
+  return l.slots * a->bank.heads * l.rows * (a->bank.dim + 2) + l.sp.want * (long)(sizeof(Split_tile) / 4);
+}
 
 template <int D, int CODE, int NS>
 void launch_attn(const rmem_bank8_attn_args& a, const Parts& parts, const Launch& l, hipStream_t s) {
@@ -870,11 +966,10 @@ int launch_dim(const rmem_bank8_attn_args& a, const Parts& parts, const Launch& 
   // a request whose row of the table holds no more than the smallest part is never divided
   if (((long)a.cols * a.bank.page + 31) / 32 > l.sp.chunk_min) {
     const long tiles = l.tiles < l.sp.want ? l.tiles : l.sp.want;       // row tiles in at least two parts: at most `want`
-    const long rows = (long)a.max_rows * l.sp.G;
-    const dim3 grid((unsigned)(tiles * a.bank.heads), (unsigned)(rows >= 1 && rows < MERGE_Y ? rows : l.rows < MERGE_Y ? l.rows : MERGE_Y));
-    if (l.rows == 16) hipLaunchKernelGGL((attn_merge<16, D>), grid, dim3(64), 0, s, a, parts, l.sp);
-    else if (l.rows == 32) hipLaunchKernelGGL((attn_merge<32, D>), grid, dim3(64), 0, s, a, parts, l.sp);
-    else hipLaunchKernelGGL((attn_merge<WROWS, D>), grid, dim3(64), 0, s, a, parts, l.sp);
+    const dim3 grid((unsigned)std::min(tiles * a.bank.heads * (l.rows / merge_block(l.rows)), 2048L));
+    if (l.rows == 16) hipLaunchKernelGGL((attn_merge<16, D>), grid, dim3(256), 0, s, a, parts, l.sp);
+    else if (l.rows == 32) hipLaunchKernelGGL((attn_merge<32, D>), grid, dim3(256), 0, s, a, parts, l.sp);
+    else hipLaunchKernelGGL((attn_merge<WROWS, D>), grid, dim3(256), 0, s, a, parts, l.sp);
     RMEM_CHECK_LAUNCH();
   }
   return RMEM_OK;
@@ -884,7 +979,9 @@ int launch_read(const rmem_bank8_attn_args& a, float* ws, const Launch& l, hipSt
   Parts parts;
   parts.o = ws;
   parts.ml = ws + l.slots * a.bank.heads * l.rows * a.bank.dim;
+  parts.tiles = reinterpret_cast<Split_tile*>(parts.ml + l.slots * a.bank.heads * l.rows * 2);
   parts.slots = (int)l.slots;
+  parts.ords = l.sp.want;
   return a.bank.dim == 32 ? launch_dim<32>(a, parts, l, s) : a.bank.dim == 64 ? launch_dim<64>(a, parts, l, s) : launch_dim<128>(a, parts, l, s);
 }
 

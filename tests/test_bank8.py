@@ -188,7 +188,7 @@ def attend_tolerance(kind, dim, out, lse, mean, most):
     """Per element.  A weight is off by a factor of e^d, d being the score's error: the product sums `dim` terms in fp32 (each
     addition at most 2^-24 of the sum of |q k|, in MFMA blocks: dim of them at worst), fp32 queries count with 22 bits (2^-22),
     the scaled score, the sum with the maximum and the exponent are rounded a few times (2^-24 of numbers below |score| + 150 in
-    the log2 domain, value scales being within 2^-96 .. 2^20) and 2^x is good to 2^-22.  Both sums see it: 2 d.  Weights are
+    the log2 domain, value scales being within 2^-88 .. 2^20) and 2^x is good to 2^-22.  Both sums see it: 2 d.  Weights are
     rounded once (2^-11; fp32 calls 2^-22, or 2^-25 of the largest weight 2^10 below the normal range), sums of weights and of
     products add fp32 roundings that are below the same terms.  Then the output's own rounding, half a step."""
     d = 2.0 ** -24 * (dim + 8) * most + (2.0 ** -22 * most if kind == "fp32" else 0) + 2.0 ** -24 * 4 * (1.4427 * np.abs(np.where(np.isfinite(lse), lse, 0)) + 20) + 2.0 ** -22
