@@ -29,20 +29,26 @@ PAGES = (32, 64, 128)
 DIMS = (32, 64, 128)
 
 
+def _refuse(what: str):
+    raise RmemError("bank8: " + what)
+
+
 def _need(ok: bool, what: str):
     if not ok:
-        raise RmemError("bank8: " + what)
+        _refuse(what)
 
 
-def _ints(t, name: str, shape, device) -> None:
-    _need(isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.device == device and tuple(t.shape) == tuple(shape) and
-          t.is_contiguous(), f"{name} must be a contiguous int32 tensor of shape {tuple(shape)} on {device}")
+def _ints(t, name: str, shape: tuple, device) -> None:
+    if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.shape == shape and t.device == device and t.is_contiguous()):
+        _refuse(f"{name} must be a contiguous int32 tensor of shape {shape} on {device}")
 
 
-def _table(t, reqs: int, device) -> None:
-    _need(isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.device == device and t.dim() == 2 and t.shape[0] == reqs and
-          t.shape[1] > 0 and t.stride(1) == 1 and (reqs == 1 or t.stride(0) >= t.shape[1]),
-          f"table must be an int32 tensor [{reqs}, pages per request] on {device} with contiguous rows")
+def _table(t, reqs: int, page: int, device) -> None:
+    if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.device == device and t.dim() == 2 and t.shape[0] == reqs and
+            t.shape[1] > 0 and t.stride(1) == 1 and (reqs == 1 or t.stride(0) >= t.shape[1])):
+        _refuse(f"table must be an int32 tensor [{reqs}, pages per request] on {device} with contiguous rows")
+    if t.shape[1] * page >= 2 ** 31:
+        _refuse("pages per request * page must be below 2^31")
 
 
 class Pool:
@@ -89,9 +95,18 @@ class Plan(NamedTuple):
     status: torch.Tensor    # [2] pages taken, pages missing
 
 
+# torch's current stream of a device as a raw pointer: what torch.cuda.current_stream(device).cuda_stream returns, without the
+# Stream object (3 us of a 15 us call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(device, name: str, args) -> None:
-    with torch.cuda.device(device):
-        hip.check(getattr(hip.load(), name)(C.byref(args), hip.stream_ptr()), name)
+    call = getattr(hip.load(), name)
+    if torch.cuda.current_device() == device.index:
+        hip.check(call(C.byref(args), _raw_stream(device.index)), name)
+    else:
+        with torch.cuda.device(device):
+            hip.check(call(C.byref(args), _raw_stream(device.index)), name)
 
 
 def plan(ctx: torch.Tensor, add: torch.Tensor, table: torch.Tensor, free: torch.Tensor, state: torch.Tensor, *, page: int, rows: int,
@@ -105,22 +120,23 @@ def plan(ctx: torch.Tensor, add: torch.Tensor, table: torch.Tensor, free: torch.
     `out` gives the results' tensors (a captured step: out.state may be `state`, out.lens may be `ctx`)."""
     _need(isinstance(ctx, torch.Tensor) and ctx.is_cuda and ctx.dim() == 1 and ctx.numel() > 0, "ctx must be a device tensor [reqs]")
     dev, reqs, rows = ctx.device, ctx.numel(), int(rows)
-    _need(page in PAGES, f"page must be one of {PAGES}")
-    _need(rows >= 0, "rows must not be negative")
-    _ints(ctx, "ctx", (reqs,), dev)
-    _ints(add, "add", (reqs,), dev)
+    _need(page in PAGES, "page must be 32, 64 or 128")
+    _need(0 <= rows < 2 ** 31, "rows must not be negative")
+    one = (reqs,)
+    _ints(ctx, "ctx", one, dev)
+    _ints(add, "add", one, dev)
     if had is not None:
-        _ints(had, "had", (reqs,), dev)
-    _table(table, reqs, dev)
-    _need(table.shape[1] * page < 2 ** 31, "pages per request * page must be below 2^31")
+        _ints(had, "had", one, dev)
+    _table(table, reqs, page, dev)
     _need(isinstance(free, torch.Tensor) and free.dim() == 1 and free.numel() > 0, "free must be a tensor [ring]")
     _ints(free, "free", (free.numel(),), dev)
     _ints(state, "state", (2,), dev)
-    sizes = dict(cu=(reqs + 1,), lens=(reqs,), start=(reqs,), slots=(rows,), state=(2,), status=(2,))
+    sizes = (reqs + 1, reqs, reqs, rows, 2, 2)          # in the order of Plan's fields
     if out is None:
-        out = Plan(*(torch.empty(sizes[n], dtype=torch.int32, device=dev) for n in Plan._fields))
-    for n in Plan._fields:
-        _ints(getattr(out, n), "out." + n, sizes[n], dev)
+        out = Plan(*torch.empty(sum(sizes), dtype=torch.int32, device=dev).split(sizes))
+    else:
+        for n, size in zip(Plan._fields, sizes):
+            _ints(getattr(out, n), "out." + n, (size,), dev)
     a = Bank8PlanArgs(ctx.data_ptr(), add.data_ptr(), hip.ptr(had), reqs, table.data_ptr(), table.stride(0) if reqs > 1 else table.shape[1],
                       table.shape[1], page, free.data_ptr(), free.numel(), state.data_ptr(), out.state.data_ptr(), out.cu.data_ptr(),
                       out.lens.data_ptr(), out.start.data_ptr(), out.slots.data_ptr(), rows, out.status.data_ptr())
@@ -129,11 +145,13 @@ def plan(ctx: torch.Tensor, add: torch.Tensor, table: torch.Tensor, free: torch.
 
 
 def _dense(t, name: str, pool: Pool, heads: int, like: Optional[torch.Tensor] = None) -> None:
-    _need(isinstance(t, torch.Tensor) and t.dim() == 3 and t.device == pool.device and t.dtype in TYPES and
-          t.shape[1] == heads and t.shape[2] == pool.dim, f"{name} must be fp32, fp16 or bf16 [rows, {heads}, {pool.dim}] on {pool.device}")
-    _need(t.stride(2) == 1 and t.stride(0) >= 0 and t.stride(1) >= 0, f"{name}'s last dimension must be contiguous")
-    if like is not None:
-        _need(t.dtype == like.dtype and t.shape == like.shape, f"{name} must have its partner's type and shape")
+    if not (isinstance(t, torch.Tensor) and t.dim() == 3 and t.device == pool.device and t.dtype in TYPES and t.shape[1] == heads and
+            t.shape[2] == pool.dim):
+        _refuse(f"{name} must be fp32, fp16 or bf16 [rows, {heads}, {pool.dim}] on {pool.device}")
+    if t.stride(2) != 1:
+        _refuse(f"{name}'s last dimension must be contiguous")
+    if like is not None and (t.dtype != like.dtype or t.shape != like.shape):
+        _refuse(f"{name} must have its partner's type and shape")
 
 
 def _workspace(given: Optional[torch.Tensor], need: int, device) -> Optional[torch.Tensor]:
@@ -141,8 +159,9 @@ def _workspace(given: Optional[torch.Tensor], need: int, device) -> Optional[tor
     _need(need >= 0, "arguments refused")
     if given is None:
         return torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    _need(isinstance(given, torch.Tensor) and given.dtype == torch.uint8 and given.is_contiguous() and given.device == device and
-          given.numel() >= need and given.data_ptr() % 16 == 0, f"workspace must be at least {need} contiguous uint8 on {device}, 16-byte aligned")
+    if not (isinstance(given, torch.Tensor) and given.dtype == torch.uint8 and given.is_contiguous() and given.device == device and
+            given.numel() >= need and given.data_ptr() % 16 == 0):
+        _refuse(f"workspace must be at least {need} contiguous uint8 on {device}, 16-byte aligned")
     return given
 
 
@@ -195,15 +214,14 @@ def attend(pool: Pool, q: torch.Tensor, cu: torch.Tensor, lens: torch.Tensor, ta
     matter.  workspace: uint8 scratch of this call alone, allocated where it is not given.
     Returns out, or (out, lse) with `with_lse` or `lse`."""
     _need(isinstance(pool, Pool), "pool must be a Pool")
-    _need(isinstance(q, torch.Tensor) and q.dim() == 3 and q.shape[1] > 0 and q.shape[1] % pool.heads == 0,
-          f"q must be [rows, a multiple of {pool.heads} heads, {pool.dim}]")
+    if not (isinstance(q, torch.Tensor) and q.dim() == 3 and q.shape[1] > 0 and q.shape[1] % pool.heads == 0):
+        _refuse(f"q must be [rows, a multiple of {pool.heads} heads, {pool.dim}]")
     _dense(q, "q", pool, q.shape[1])
     _need(isinstance(lens, torch.Tensor) and lens.dim() == 1 and lens.numel() > 0, "lens must be a tensor [reqs]")
     dev, reqs, rows, heads_q = pool.device, lens.numel(), q.shape[0], q.shape[1]
     _ints(lens, "lens", (reqs,), dev)
     _ints(cu, "cu", (reqs + 1,), dev)
-    _table(table, reqs, dev)
-    _need(table.shape[1] * pool.page < 2 ** 31, "pages per request * page must be below 2^31")
+    _table(table, reqs, pool.page, dev)
     scale = 1.0 / math.sqrt(pool.dim) if scale is None else float(scale)
     _need(0.0 < scale < 3e38, "scale must be positive and finite")
     if out is None:
@@ -217,7 +235,7 @@ def attend(pool: Pool, q: torch.Tensor, cu: torch.Tensor, lens: torch.Tensor, ta
         lse = torch.empty((rows, heads_q), dtype=torch.float32, device=dev)
     a = Bank8AttnArgs(pool.args, q.data_ptr(), out.data_ptr(), hip.ptr(lse), TYPES[q.dtype], q.stride(0), q.stride(1), out.stride(0),
                       out.stride(1), cu.data_ptr(), lens.data_ptr(), reqs, rows, table.data_ptr(),
-                      table.stride(0) if reqs > 1 else table.shape[1], table.shape[1], heads_q, rows if max_q is None else int(max_q),
+                      table.stride(0) if reqs > 1 else table.shape[1], table.shape[1], heads_q, rows if max_q is None else min(max(int(max_q), 0), 2 ** 31 - 1),
                       int(bool(causal)), scale, None, 0)
     if rows:
         ws = _workspace(workspace, hip.load().rmem_bank8_attn_workspace(C.byref(a)), dev)

@@ -43,40 +43,45 @@ __device__ __forceinline__ frag8_t decode8(uint32_t u0, uint32_t u1) {
   return __builtin_bit_cast(frag8_t, w);
 }
 
-__device__ __forceinline__ float decode1(uint32_t byte, int code) {
-  if (code == INT8) return (float)(int)byte - 128.f;
-  const f16x2_t h = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(byte, 1.0f, false);
-  return (float)h[0];
-}
-// x in units of the scale -> code byte, round to nearest even, saturating; NaN -> 0
-__device__ __forceinline__ uint32_t encode1(float x, int code) {
+// Four numbers in units of the scale -> four code bytes: round to nearest even, saturating, NaN -> 0.  int8: adding 1.5 * 2^23 + 128
+// leaves the rounded number + 128 in the low byte.
+__device__ __forceinline__ float clean(float x, float top) {
   x = x == x ? x : 0.f;
-  if (code == INT8) return (uint32_t)((int)rintf(fminf(fmaxf(x, -127.f), 127.f)) + 128);
-  x = fminf(fmaxf(x, -448.f), 448.f);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x, 0.f, 0, false) & 0xffu;
+  return __builtin_amdgcn_fmed3f(x, -top, top);
 }
-__device__ __forceinline__ uint32_t zero_code(int code) { return code == INT8 ? 128u : 0u; }
-__device__ __forceinline__ float code_top(int code) { return code == INT8 ? 127.f : 448.f; }
-
-template <int T>
-struct Elem;
-template <>
-struct Elem<FP32> { typedef float type; };
-template <>
-struct Elem<FP16> { typedef _Float16 type; };
-template <>
-struct Elem<BF16> { typedef __bf16 type; };
-
-__device__ __forceinline__ float load1(const void* p, long i, int type) {
-  if (type == FP32) return static_cast<const float*>(p)[i];
-  if (type == FP16) return (float)static_cast<const _Float16*>(p)[i];
-  return (float)static_cast<const __bf16*>(p)[i];
+template <int CODE>
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+  if constexpr (CODE == INT8) {
+    const uint32_t x = __float_as_uint(clean(a, 127.f) + 12583040.f), y = __float_as_uint(clean(b, 127.f) + 12583040.f),
+                   z = __float_as_uint(clean(c, 127.f) + 12583040.f), w = __float_as_uint(clean(d, 127.f) + 12583040.f);
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(w, z, 0x0c0c0400u), __builtin_amdgcn_perm(y, x, 0x0c0c0400u), 0x05040100u);
+  } else {
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(clean(a, 448.f), clean(b, 448.f), 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(clean(c, 448.f), clean(d, 448.f), lo, true);
+  }
 }
-__device__ __forceinline__ void store1(void* p, long i, float x, int type) {
-  if (type == FP32) static_cast<float*>(p)[i] = x;
-  else if (type == FP16) static_cast<_Float16*>(p)[i] = (_Float16)x;
-  else static_cast<__bf16*>(p)[i] = (__bf16)x;
+// four code bytes -> their values
+template <int CODE>
+__device__ __forceinline__ f32x4_t values4(uint32_t u) {
+  f32x4_t x;
+  if constexpr (CODE == INT8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = (float)((u >> (8 * i)) & 0xffu) - 128.f;
+  } else {
+    uint32_t a, b;
+    decode4<CODE>(u, a, b);
+    const f16x2_t p = __builtin_bit_cast(f16x2_t, a), q = __builtin_bit_cast(f16x2_t, b);
+    x[0] = (float)p[0]; x[1] = (float)p[1]; x[2] = (float)q[0]; x[3] = (float)q[1];
+  }
+  return x;
 }
+template <int CODE>
+__device__ __forceinline__ uint32_t recode4(uint32_t u, float ratio) {       // codes of a page whose scale has risen
+  const f32x4_t x = values4<CODE>(u) * ratio;
+  return encode4<CODE>(x[0], x[1], x[2], x[3]);
+}
+template <int CODE>
+__device__ __forceinline__ uint32_t zeros4() { return CODE == INT8 ? 0x80808080u : 0u; }
 
 // Argument checks shared by the entry points (no HIP call: they run without a GPU).
 inline bool valid_bank(const rmem_bank8* b) {

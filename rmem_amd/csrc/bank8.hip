@@ -2,12 +2,15 @@
 // Storage and semantics: include/rmem_hip.h and bank8.h; the read over the pages is bank8_attn.hip.
 #include "bank8.h"
 
+#include <algorithm>
+#include <type_traits>
+
 using namespace bank8;
 
 namespace {
 
 // ------------------------------------------------------------------------------------------------------------------- plan
-// One workgroup: the requests are scanned (pages asked for, rows, pages going back) a chunk of 1024 at a time, the page ids that
+// One workgroup: the requests are scanned (pages asked for, rows, pages going back) up to 1024 at a time, the page ids that
 // move are spread over the threads by binary search in the scan.  Bound by the chain of dependent memory reads (lengths -> ring
 // and table entries), not by bytes; one workgroup keeps it one launch and lets state and lengths be updated in place.
 constexpr int PT = 1024;
@@ -43,14 +46,16 @@ __global__ __launch_bounds__(PT) void plan_kernel(rmem_bank8_plan_args p, int ps
   __shared__ int s_held[PT], s_start[PT], s_rel[PT];
   __shared__ long long s_wave[3][PT / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int page_mask = (1 << ps) - 1;
+  const int page_mask = (1 << ps) - 1, threads = blockDim.x;
   int head = p.state_in[0], count = p.state_in[1];
-  head = p.ring > 0 ? (int)(((long long)head % p.ring + p.ring) % p.ring) : 0;
+  head %= p.ring;
+  head += head < 0 ? p.ring : 0;
   count = count < 0 ? 0 : count > p.ring ? p.ring : count;
+  auto ring_at = [&](long long i) { const long long at = head + i; return at >= p.ring ? at - p.ring : at; };   // i < ring
   long long c_need = 0, c_rows = 0, c_back = 0;              // carried from earlier chunks
   long long taken = 0, missing = 0;                          // this thread's requests
   const bool inline_slots = p.rows <= SLOTS_INLINE;
-  for (int base = 0; base < p.reqs; base += PT) {
+  for (int base = 0; base < p.reqs; base += threads) {
     const int r = base + tid;
     long long ctx = 0, add = 0, need = 0, asked = 0, back = 0, held = 0;
     bool fits = false;
@@ -103,33 +108,33 @@ __global__ __launch_bounds__(PT) void plan_kernel(rmem_bank8_plan_args p, int ps
       if (r == 0) p.cu[0] = 0;
     }
     __syncthreads();
-    const int nr = p.reqs - base < PT ? p.reqs - base : PT;
+    const int nr = min(p.reqs - base, threads);
     const long long n_need = s_need[nr - 1], n_rows = s_rows[nr - 1], n_back = s_back[nr - 1];
     // pages going back, before new entries can overwrite them in the table
-    for (long long i = tid; i < n_back; i += PT) {
+    for (long long i = tid; i < n_back; i += threads) {
       const int k = upper_bound(s_back, nr, i);
       const long long j = i - (k ? s_back[k - 1] : 0);
       const long long at = count + c_back + i;
       if (at < p.ring)                                       // (more pages than the ring holds: returned twice, dropped)
-        p.free_ring[(head + at) % p.ring] = p.table[(base + k) * p.ld_table + s_held[k] + j];
+        p.free_ring[ring_at(at)] = p.table[(base + k) * p.ld_table + s_held[k] + j];
     }
     if (n_back) __syncthreads();
-    for (long long i = tid; i < n_need; i += PT) {
+    for (long long i = tid; i < n_need; i += threads) {
       const int k = upper_bound(s_need, nr, i);
       const long long j = i - (k ? s_need[k - 1] : 0);
-      if (s_start[k] >= 0) p.table[(base + k) * p.ld_table + s_held[k] + j] = p.free_ring[(head + c_need + i) % p.ring];
+      if (s_start[k] >= 0) p.table[(base + k) * p.ld_table + s_held[k] + j] = p.free_ring[ring_at(c_need + i)];
     }
     if (inline_slots) {
       // rows of this chunk; entries are taken from where they come from, so nothing waits for the table's writes
       const long long end = c_rows + n_rows < p.rows ? c_rows + n_rows : p.rows;
-      for (long long t = c_rows + tid; t < end; t += PT) {
+      for (long long t = c_rows + tid; t < end; t += threads) {
         const int k = upper_bound(s_rows, nr, t - c_rows);
         const int start = s_start[k];
         int slot = -1;
         if (start >= 0) {
           const long long pos = start + (t - c_rows) - (k ? s_rows[k - 1] : 0);
           const long long pi = pos >> ps;
-          const int id = pi >= s_held[k] ? p.free_ring[(head + c_need + (k ? s_need[k - 1] : 0) + pi - s_held[k]) % p.ring]
+          const int id = pi >= s_held[k] ? p.free_ring[ring_at(c_need + (k ? s_need[k - 1] : 0) + pi - s_held[k])]
                                          : p.table[(base + k) * p.ld_table + pi];
           slot = slot_of(id, pos, ps);
         }
@@ -142,7 +147,7 @@ __global__ __launch_bounds__(PT) void plan_kernel(rmem_bank8_plan_args p, int ps
     __syncthreads();                                         // the chunk's sums are overwritten next
   }
   if (inline_slots)
-    for (long long t = c_rows + tid; t < p.rows; t += PT) p.slots[t] = -1;
+    for (long long t = c_rows + tid; t < p.rows; t += threads) p.slots[t] = -1;
   // totals
   long long x = taken, y = missing;
 #pragma unroll
@@ -160,12 +165,12 @@ __global__ __launch_bounds__(PT) void plan_kernel(rmem_bank8_plan_args p, int ps
   __syncthreads();
   if (tid == 0) {
     long long t = 0, m = 0;
-    for (int w = 0; w < PT / 64; ++w) {
+    for (int w = 0; w < threads / 64; ++w) {
       t += s_wave[0][w];
       m += s_wave[1][w];
     }
     const long long left = count - t + c_back;
-    p.state_out[0] = p.ring > 0 ? (int)((head + t) % p.ring) : 0;
+    p.state_out[0] = (int)(head + t >= p.ring ? head + t - p.ring : head + t);
     p.state_out[1] = (int)(left < p.ring ? left : p.ring);
     p.status[0] = (int)t;
     p.status[1] = (int)(m < 0x7fffffff ? m : 0x7fffffff);
@@ -203,6 +208,7 @@ __device__ __forceinline__ float finite_abs(float x) {
 // (16 KB at most, from the L2); beyond, two small launches mark each page's first row and count its runs, and only a page that is
 // reached by several runs is searched for.
 constexpr int SCAN_ROWS = 4096;
+constexpr int APPEND_GROUPS = 4096;      // workgroups from which on a workgroup takes several rows
 
 __device__ __forceinline__ bool in_pool(int slot, const rmem_bank8& b) { return slot >= 0 && slot < b.pages * (long)b.page; }
 // whether `row` goes on where the row before it ended, in the same page
@@ -230,156 +236,315 @@ __global__ __launch_bounds__(256) void mark_kernel(rmem_bank8_append_args a, Pag
   atomicAdd(&marks[slot >> ps].runs, 1);
 }
 
-// One workgroup per (row, head, keys or values).
-__global__ __launch_bounds__(256) void append_kernel(rmem_bank8_append_args a, const PageMark* marks, int ps) {
+// N elements as they lie in memory: one vector (or several of 16 bytes) with WIDE.  Loads are issued for all of a
+// thread's places, rows that do not exist reading one that does: a branch around a load ends in a wait for it.
+template <class T, int N, bool WIDE>
+struct Run {
+  static constexpr int V = !WIDE ? 1 : N < 16 / (int)sizeof(T) ? N : 16 / (int)sizeof(T);
+  typedef __attribute__((ext_vector_type(V))) T vec_t;
+  vec_t y[N / V];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int k = 0; k < N / V; ++k) y[k] = *reinterpret_cast<const vec_t*>(p + k * V);
+  }
+  __device__ __forceinline__ float at(int e) const { return (float)y[e / V][e % V]; }
+};
+// element `at` of row r: with FAST a 32-bit byte offset from the (uniform) base, one register instead of two for each of a
+// thread's loads in flight
+template <class T, bool FAST>
+__device__ __forceinline__ const T* element(const T* src, long ldr, int r, int at) {
+  if constexpr (FAST) return reinterpret_cast<const T*>(reinterpret_cast<const char*>(src) + ((unsigned)r * (unsigned)ldr + (unsigned)at) * (unsigned)sizeof(T));
+  else return src + r * ldr + at;
+}
+
+// One workgroup per (window of rows, head, keys or values); each page that begins in the window (its first row in the call lies
+// there) is read twice, for its largest value and, from the caches, to be encoded: holding it in registers in between (64 to 128 of
+// them) leaves too few workgroups to hide the chain slots -> rows -> maximum -> codes.  Keys: a thread takes 16 dims of a token,
+// eight threads a token of 128 dims (256 bytes in, 128-byte pieces out).  Values: a thread takes 16 tokens (half a 32-token tile)
+// of two dims, so that a wave reads whole rows and each thread writes the two chunks that hold its tokens.
+template <class T, int CODE, int D, bool FAST>
+__global__ __launch_bounds__(256, 4) void append_kernel(rmem_bank8_append_args a, const PageMark* marks, int ps, int window) {
   __shared__ float s_max[4];
-  __shared__ int s_row[128];              // row that fills each place of the page, -1: none; the last of several
-  __shared__ int s_end[2];                // one past the last place filled, and the complement of the first
+  __shared__ __attribute__((aligned(16))) int s_row[128];   // row that fills each place of the page, -1: none; the last of several
   __shared__ int s_other;
-  const int row = blockIdx.x, h = blockIdx.y, part = blockIdx.z;
+  const int h = blockIdx.y, part = blockIdx.z;
   const rmem_bank8& b = a.bank;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int page = b.page, dim = b.dim, code = b.code;
-  const int slot = a.slots[row];
-  if (!in_pool(slot, b) || goes_on(a.slots, row, slot, page)) return;
-  const int pg32 = slot >> ps;
-  int runs = 0;
-  if (marks) {
-    if (marks[pg32].first != row) return;
-    runs = marks[pg32].runs;
-  }
-  if (tid < 128) s_row[tid] = -1;
-  if (tid < 2) s_end[tid] = 0;
-  if (tid == 0) s_other = 0;
-  __syncthreads();
-  if (runs == 1) {
-    const long r = (long)row + tid;
-    const int at = (slot & (page - 1)) + tid;
-    if (at < page && r < a.rows) {
-      // the run ends where the slots do not go on: later rows that fit the pattern again would be a second run
-      if (a.slots[r] == slot + tid) s_row[at] = (int)r;
-    }
-  } else {
-    for (int r = marks ? row + tid : tid; r < a.rows; r += 256) {
-      const int s = a.slots[r];
-      if (s < 0 || (s >> ps) != pg32) continue;
-      if (r < row) s_other = 1;
-      else atomicMax(&s_row[s & (page - 1)], r);
+  const int page = b.page;
+  const T* src = static_cast<const T*>(part ? a.v : a.k) + (long)h * (part ? a.v_head : a.k_head);
+  const long ldr = part ? a.v_row : a.k_row;
+  // every wave looks the window's rows over at once: which of them begin a page that is this workgroup's to write
+  const int row0 = blockIdx.x * window;
+  int w_slot = -1, w_runs = 0;
+  bool begins = false;
+  if (lane < window && row0 + lane < a.rows) {
+    w_slot = a.slots[row0 + lane];
+    begins = in_pool(w_slot, b) && !goes_on(a.slots, row0 + lane, w_slot, page);
+    if (marks && begins) {
+      const PageMark m = marks[w_slot >> ps];
+      begins = m.first == row0 + lane;
+      w_runs = m.runs;
     }
   }
-  __syncthreads();
-  if (s_other) return;
-  if (tid < page && s_row[tid] >= 0) {
-    atomicMax(&s_end[0], tid + 1);
-    atomicMax(&s_end[1], 128 - tid);
-  }
-  __syncthreads();
-  const int hi = s_end[0], lo = 128 - s_end[1];
-
-  const long pg = pg32;
-  const void* src = part ? a.v : a.k;
-  const long ldr = part ? a.v_row : a.k_row, base = (long)h * (part ? a.v_head : a.k_head);
-  uint8_t* codes = (part ? b.v : b.k) + (pg * b.heads + h) * ((long)page * dim);
-  float* scale_p = (part ? b.v_scale : b.k_scale) + pg * b.heads + h;
-
-  float mx = 0.f;
-  for (int i = tid; i < (hi - lo) * dim; i += 256) {
-    const int r = s_row[lo + i / dim];
-    if (r >= 0) mx = fmaxf(mx, finite_abs(load1(src, base + r * ldr + i % dim, a.type)));
-  }
-  mx = wave_max_xor(mx);
-  if (lane == 0) s_max[wave] = mx;
-  const float was = lo ? *scale_p : 0.f;
-  __syncthreads();
-  mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-  const float fresh = fmaxf(mx, 1e-30f) / code_top(code);
-  const bool grown = lo && fresh > was;
-  const float scale = lo && !grown ? was : fresh;
-  const float inv = 1.0f / scale, ratio = grown ? was / scale : 1.0f;
-  if (tid == 0) *scale_p = scale;                             // (every thread has read it: the barrier above)
-
-  // Places that no row fills: in front of and between new tokens of a page that kept some, their codes stay (rounded again where
-  // the scale rose); in a page that begins anew they become 0.
-  if (!part) {
-    // unit: 16 dims of a token
-    const int first = grown ? 0 : lo, n = hi - first;
-    for (int i = tid; i < n * (dim / 16); i += 256) {
-      const int key = first + i % n, c = i / n, r = s_row[key];
-      if (r < 0 && lo && !grown) continue;
-      u32x4_t* dst = reinterpret_cast<u32x4_t*>(codes + ((long)c * page + key) * 16);
-      u32x4_t w;
-      if (r >= 0) {
-        const long at = base + r * ldr + c * 16;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t u = 0;
-#pragma unroll
-          for (int f = 0; f < 4; ++f) u |= encode1(load1(src, at + 4 * e + f, a.type) * inv, code) << (8 * f);
-          w[e] = u;
-        }
-      } else if (lo) {
-        w = *dst;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t u = 0;
-#pragma unroll
-          for (int f = 0; f < 4; ++f) u |= encode1(decode1((w[e] >> (8 * f)) & 0xff, code) * ratio, code) << (8 * f);
-          w[e] = u;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = 0x01010101u * zero_code(code);
+  for (unsigned long long todo = __ballot(begins); todo; todo &= todo - 1) {
+    const int at0 = __builtin_ctzll(todo), row = row0 + at0;
+    const int slot = __builtin_amdgcn_readlane(w_slot, at0), runs = __builtin_amdgcn_readlane(w_runs, at0);
+    const int pg32 = slot >> ps, off = slot & (page - 1);
+    float* scale_p = (part ? b.v_scale : b.k_scale) + (long)pg32 * b.heads + h;
+    const float before = *scale_p;
+    __syncthreads();                      // the page before has been written
+    if (runs == 1) {
+      // the run goes on where the slots do; a row further on that fitted the pattern again would begin another run
+      const long r = (long)row + tid - off;
+      if (tid < 128) s_row[tid] = tid >= off && tid < page && r < a.rows && a.slots[r] == slot + tid - off ? (int)r : -1;
+      if (tid == 0) s_other = 0;
+    } else {
+      if (tid < 128) s_row[tid] = -1;
+      if (tid == 0) s_other = 0;
+      __syncthreads();
+      for (int r = marks ? row + tid : tid; r < a.rows; r += 256) {
+        const int s = a.slots[r];
+        if (s < 0 || (s >> ps) != pg32) continue;
+        if (r < row) s_other = 1;
+        else atomicMax(&s_row[s & (page - 1)], r);
       }
-      *dst = w;
     }
-  } else {
-    // unit: 16 tokens of a dim (half a 32-token tile)
-    const int t0 = grown ? 0 : lo >> 5, t1 = (hi + 31) >> 5;
-    for (int i = tid; i < (t1 - t0) * 2 * dim; i += 256) {
-      const int d = i % dim, th = i / dim, tile = t0 + (th >> 1), half = th & 1;
-      u32x4_t* dst = reinterpret_cast<u32x4_t*>(codes + (((long)tile * 2 + half) * dim + d) * 16);
-      u32x4_t w = *dst;
+    __syncthreads();
+    if (s_other) continue;
+    // places filled: first, one past the last, whether there are gaps
+    const unsigned long long f0 = __ballot(s_row[lane] >= 0), f1 = __ballot(s_row[64 + lane] >= 0);
+    const int lo = f0 ? __builtin_ctzll(f0) : 64 + __builtin_ctzll(f1), hi = f1 ? 128 - __builtin_clzll(f1) : 64 - __builtin_clzll(f0);
+    const bool holes = __popcll(f0) + __popcll(f1) < hi - lo;
+
+    uint8_t* codes = (part ? b.v : b.k) + ((long)pg32 * b.heads + h) * ((long)page * D);
+    // the new tokens' largest value, four loads of eight elements in flight per thread
+    float mx = 0.f;
+    constexpr int W = D / 8;
+    for (int u0 = tid; u0 < (hi - lo) * W; u0 += 4 * 256) {
+      Run<T, 8, FAST> y[4];
+      int r[4];
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        uint32_t u = 0;
-#pragma unroll
-        for (int f = 0; f < 4; ++f) {
-          const int key = tile * 32 + 8 * m + 4 * half + f, r = s_row[key];
-          uint32_t x = (w[m] >> (8 * f)) & 0xff;
-          if (r >= 0) x = encode1(load1(src, base + r * ldr + d, a.type) * inv, code);
-          else if (key >= hi || !lo) x = zero_code(code);
-          else if (grown) x = encode1(decode1(x, code) * ratio, code);
-          u |= x << (8 * f);
-        }
-        w[m] = u;
+      for (int i = 0; i < 4; ++i) {
+        const int u = u0 + i * 256, place = lo + u / W;
+        r[i] = place < hi ? s_row[place] : -1;
+        y[i].load(element<T, FAST>(src, ldr, r[i] < 0 ? row : r[i], (u % W) * 8));
       }
-      *dst = w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, r[i] < 0 ? 0.f : finite_abs(y[i].at(e)));
+    }
+    mx = wave_max_xor(mx);
+    if (lane == 0) s_max[wave] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+    const float was = lo ? before : 0.f, fresh = fmaxf(mx, 1e-30f) / (CODE == INT8 ? 127.f : 448.f);
+    const bool grown = lo && fresh > was;
+    const float scale = lo && !grown ? was : fresh;
+    const float inv = 1.0f / scale, ratio = grown ? was / scale : 1.0f;
+    if (tid == 0) *scale_p = scale;                 // (every thread has read it: the barriers above)
+
+    // Places that no row fills: in front of and between new tokens of a page that kept some, their codes stay (rounded again where
+    // the scale rose); in a page that begins anew they become 0.
+    if (!part) {
+      constexpr int C = D / 16;
+      auto at = [&](int key, int c) { return reinterpret_cast<u32x4_t*>(codes + ((long)c * page + key) * 16); };
+      for (int u0 = tid; u0 < (hi - lo) * C; u0 += 2 * 256) {
+        Run<T, 16, FAST> y[2];
+        int r[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int u = u0 + i * 256, key = lo + u / C;
+          r[i] = key < hi ? s_row[key] : -1;
+          y[i].load(element<T, FAST>(src, ldr, r[i] < 0 ? row : r[i], (u % C) * 16));
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int u = u0 + i * 256;
+          if (r[i] < 0) continue;
+          u32x4_t w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            w[e] = encode4<CODE>(y[i].at(4 * e) * inv, y[i].at(4 * e + 1) * inv, y[i].at(4 * e + 2) * inv, y[i].at(4 * e + 3) * inv);
+          *at(lo + u / C, u % C) = w;
+        }
+      }
+      if (grown || (holes && !lo))
+        for (int u = tid; u < hi * C; u += 256) {
+          const int key = u / C;
+          if (s_row[key] >= 0) continue;
+          u32x4_t w = *at(key, u % C);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = grown ? recode4<CODE>(w[e], ratio) : zeros4<CODE>();
+          *at(key, u % C) = w;
+        }
+    } else {
+      constexpr int P = D / 2;
+      const int t0 = lo >> 5, t1 = (hi + 31) >> 5;
+      auto at = [&](int th, int d) { return reinterpret_cast<u32x4_t*>(codes + ((long)th * D + d) * 16); };
+      for (int u = 2 * t0 * P + tid; u < 2 * t1 * P; u += 256) {
+        const int th = u / P, d = 2 * (u % P);
+        Run<T, 2, FAST> y[16];
+        uint32_t fill[4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const int4 r = *reinterpret_cast<const int4*>(&s_row[(th >> 1) * 32 + 8 * m + 4 * (th & 1)]);
+          fill[m] = (r.x >= 0 ? 0xffu : 0u) | (r.y >= 0 ? 0xff00u : 0u) | (r.z >= 0 ? 0xff0000u : 0u) | (r.w >= 0 ? 0xff000000u : 0u);
+          y[4 * m].load(element<T, FAST>(src, ldr, r.x < 0 ? row : r.x, d));
+          y[4 * m + 1].load(element<T, FAST>(src, ldr, r.y < 0 ? row : r.y, d));
+          y[4 * m + 2].load(element<T, FAST>(src, ldr, r.z < 0 ? row : r.z, d));
+          y[4 * m + 3].load(element<T, FAST>(src, ldr, r.w < 0 ? row : r.w, d));
+        }
+        u32x4_t w[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+        if (lo && ((th >> 1) * 32 < lo || holes)) {
+          w[0] = *at(th, d);
+          w[1] = *at(th, d + 1);
+        }
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const int n = hi - ((th >> 1) * 32 + 8 * m + 4 * (th & 1));      // places below hi of these four
+          const uint32_t below = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u, keep = lo ? below & ~fill[m] : 0u;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t now = encode4<CODE>(y[4 * m].at(k) * inv, y[4 * m + 1].at(k) * inv, y[4 * m + 2].at(k) * inv, y[4 * m + 3].at(k) * inv);
+            const uint32_t kept = grown ? recode4<CODE>(w[k][m], ratio) : w[k][m];
+            w[k][m] = (now & fill[m]) | (kept & keep) | (zeros4<CODE>() & ~(fill[m] | keep));
+          }
+        }
+        *at(th, d) = w[0];
+        *at(th, d + 1) = w[1];
+      }
+      if (grown)
+        for (int u = tid; u < 2 * t0 * D; u += 256) {
+          u32x4_t w = *at(u / D, u % D);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = recode4<CODE>(w[e], ratio);
+          *at(u / D, u % D) = w;
+        }
     }
   }
 }
 
 // ----------------------------------------------------------------------------------------------------------------- gather
-// One thread: 16 dims of a (row, head), keys and values.
-__global__ __launch_bounds__(256) void gather_kernel(rmem_bank8_gather_args a, int ps) {
+// One wave per (32 rows, head, keys or values).  Keys: D / 16 lanes per row, 16 dims each.  Values lie by tokens, so consecutive
+// rows of one 32-token tile are read together: a lane takes two dims of half the tile, 32 bytes, and writes its tokens' pairs.
+template <class T, int CODE, int D>
+__global__ __launch_bounds__(64) void gather_kernel(rmem_bank8_gather_args a, int ps) {
   const rmem_bank8& b = a.bank;
-  const int chunks = b.dim / 16;
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (long)a.rows * b.heads * chunks) return;
-  const int c = (int)(i % chunks), h = (int)(i / chunks % b.heads);
-  const long row = i / chunks / b.heads;
-  const int slot = a.slots[row];
-  const bool in = slot >= 0 && slot < b.pages * (long)b.page;
-  const long pg = in ? slot >> ps : 0, at = pg * b.heads + h;
-  const int key = in ? slot & (b.page - 1) : 0, q = key & 31;
-  const float ks = in ? b.k_scale[at] : 0.f, vs = in ? b.v_scale[at] : 0.f;
-  const uint8_t* k = b.k + at * ((long)b.page * b.dim) + ((long)c * b.page + key) * 16;
-  const uint8_t* v = b.v + at * ((long)b.page * b.dim) + (((long)(key >> 5) * 2 + ((q >> 2) & 1)) * b.dim + c * 16) * 16 + 4 * (q >> 3) + (q & 3);
-  const long o = i * 16;
-  for (int e = 0; e < 16; ++e) {
-    store1(a.ko, o + e, in ? decode1(k[e], b.code) * ks : 0.f, a.type);
-    store1(a.vo, o + e, in ? decode1(v[e * 16], b.code) * vs : 0.f, a.type);
+  const int lane = threadIdx.x, h = blockIdx.y, page = b.page;
+  const int row0 = blockIdx.x * 32, nr = min(32, a.rows - row0);
+  int slot = -1;
+  if (lane < nr) {
+    slot = a.slots[row0 + lane];
+    if (!in_pool(slot, b)) slot = -1;
+  }
+  const long pstride = (long)b.heads * page * D;
+  float scale = 0.f;
+  if (slot >= 0) scale = (blockIdx.z ? b.v_scale : b.k_scale)[(long)(slot >> ps) * b.heads + h];
+  if (blockIdx.z == 0) {
+    constexpr int C = D / 16, R = 64 / C, N = 32 / R;         // lanes per row, rows at once, steps
+    const int c = lane % C;
+    const uint8_t* codes = b.k + (long)h * page * D;
+    u32x4_t w[N];
+    float sc[N];
+    int s[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = i * R + lane / C;
+      s[i] = __shfl(slot, r);
+      sc[i] = __shfl(scale, r);
+      w[i] = u32x4_t{0, 0, 0, 0};
+      if (s[i] >= 0) w[i] = *reinterpret_cast<const u32x4_t*>(codes + (s[i] >> ps) * pstride + (c * page + (s[i] & (page - 1))) * 16);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = i * R + lane / C;
+      if (r >= nr) continue;
+      typedef __attribute__((ext_vector_type(16 / sizeof(T)))) T vec_t;
+      constexpr int V = 16 / sizeof(T);
+      vec_t y[16 / V];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const f32x4_t x = values4<CODE>(w[i][e]) * sc[i];
+#pragma unroll
+        for (int f = 0; f < 4; ++f) y[(4 * e + f) / V][(4 * e + f) % V] = (T)(s[i] >= 0 ? x[f] : 0.f);
+      }
+      T* out = static_cast<T*>(a.ko) + ((long)(row0 + r) * b.heads + h) * D + c * 16;
+#pragma unroll
+      for (int k = 0; k < 16 / V; ++k) *reinterpret_cast<vec_t*>(out + k * V) = y[k];
+    }
+  } else {
+    typedef __attribute__((ext_vector_type(2))) T pair_t;
+    const int before = __shfl_up(slot, 1);
+    const bool first = lane == 0 || slot < 0 || before < 0 || slot != before + 1 || (slot & 31) == 0;
+    unsigned long long starts = __ballot(first && lane < nr);
+    const uint8_t* codes = b.v + (long)h * page * D;
+    T* out = static_cast<T*>(a.vo) + ((long)row0 * b.heads + h) * D;
+    const long ldo = (long)b.heads * D;
+    while (starts) {
+      const int i0 = __builtin_ctzll(starts);
+      starts &= starts - 1;
+      const int i1 = starts ? __builtin_ctzll(starts) : nr;
+      const int s = __builtin_amdgcn_readlane(slot, i0);
+      const float sc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scale), i0));
+      if (s < 0) {                                            // (rows outside the pool are segments of one)
+        for (int d = 2 * lane; d < D; d += 128) *reinterpret_cast<pair_t*>(out + i0 * ldo + d) = pair_t{(T)0.f, (T)0.f};
+        continue;
+      }
+      const int key0 = s & 31;
+      const uint8_t* tile = codes + (s >> ps) * pstride + (long)((s & (page - 1)) >> 5) * (32 * D);
+#pragma unroll
+      for (int u0 = 0; u0 < D; u0 += 64) {
+        const int u = u0 + lane, half = u / (D / 2), d = 2 * (u % (D / 2));
+        if (u >= D) break;
+        const u32x4_t* p = reinterpret_cast<const u32x4_t*>(tile + (half * D + d) * 16);
+        const u32x4_t w0 = p[0], w1 = p[1];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const f32x4_t x = values4<CODE>(w0[m]) * sc, y = values4<CODE>(w1[m]) * sc;
+#pragma unroll
+          for (int f = 0; f < 4; ++f) {
+            const int r = i0 + 8 * m + 4 * half + f - key0;
+            if (r >= i0 && r < i1) *reinterpret_cast<pair_t*>(out + r * ldo + d) = pair_t{(T)x[f], (T)y[f]};
+          }
+        }
+      }
+    }
   }
 }
+
+// kernels by type, code and dim
+template <template <class, int, int> class F, class... A>
+void dispatch(int type, int code, int dim, A&&... args) {
+  auto dims = [&](auto t, auto c) {
+    typedef decltype(t) T;
+    constexpr int CODE = decltype(c)::value;
+    if (dim == 32) F<T, CODE, 32>::run(args...);
+    else if (dim == 64) F<T, CODE, 64>::run(args...);
+    else F<T, CODE, 128>::run(args...);
+  };
+  auto codes = [&](auto t) { code == INT8 ? dims(t, std::integral_constant<int, INT8>()) : dims(t, std::integral_constant<int, E4M3>()); };
+  if (type == FP32) codes(float());
+  else if (type == FP16) codes((_Float16)0.f);
+  else codes((__bf16)0.f);
+}
+template <class T, int CODE, int D>
+struct Append {
+  static void run(const rmem_bank8_append_args& a, const PageMark* marks, int ps, int window, hipStream_t s) {
+    // FAST: every row of every head begins on 16 bytes, and the rows span less than 4 GiB
+    const unsigned long mis = (unsigned long)a.k | (unsigned long)a.v | (unsigned long)((a.k_row | a.k_head | a.v_row | a.v_head) * (long)sizeof(T));
+    const dim3 grid((a.rows + window - 1) / window, a.bank.heads, 2);
+    const long span = (a.rows - 1L) * std::max(a.k_row, a.v_row) + D;
+    if ((mis & 15) || span * (long)sizeof(T) >= 1L << 32) hipLaunchKernelGGL((append_kernel<T, CODE, D, false>), grid, dim3(256), 0, s, a, marks, ps, window);
+    else hipLaunchKernelGGL((append_kernel<T, CODE, D, true>), grid, dim3(256), 0, s, a, marks, ps, window);
+  }
+};
+template <class T, int CODE, int D>
+struct Gather {
+  static void run(const rmem_bank8_gather_args& a, int ps, hipStream_t s) {
+    hipLaunchKernelGGL((gather_kernel<T, CODE, D>), dim3((a.rows + 31) / 32, a.bank.heads, 2), dim3(64), 0, s, a, ps);
+  }
+};
 
 }  // namespace
 
@@ -390,7 +555,9 @@ extern "C" int rmem_bank8_plan(const rmem_bank8_plan_args* a, void* stream) {
     return RMEM_ERR_INVALID;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int ps = log2_of(a->page);
-  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(PT), 0, s, *a, ps);
+  // as many threads as the requests, or a quarter of the rows, can use: a step of few requests is one wave and no barrier's wait
+  const int use = std::max(a->reqs, a->rows <= SLOTS_INLINE ? a->rows / 4 : PT), threads = use >= PT ? PT : use <= 64 ? 64 : (use + 63) & ~63;
+  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(threads), 0, s, *a, ps);
   RMEM_CHECK_LAUNCH();
   if (a->rows > SLOTS_INLINE) {
     hipLaunchKernelGGL(slots_kernel, dim3((unsigned)(((long)a->rows + 255) / 256)), dim3(256), 0, s, *a, ps);
@@ -400,7 +567,8 @@ extern "C" int rmem_bank8_plan(const rmem_bank8_plan_args* a, void* stream) {
 }
 
 static bool valid_append(const rmem_bank8_append_args* a) {
-  return a && valid_bank(&a->bank) && valid_type(a->type) && a->rows >= 0 && a->rows < 1 << 24 && a->bank.heads <= 65535;
+  return a && valid_bank(&a->bank) && valid_type(a->type) && a->rows >= 0 && a->rows < 1 << 24 && a->bank.heads <= 65535 && a->k_row >= 0 &&
+         a->k_head >= 0 && a->v_row >= 0 && a->v_head >= 0;
 }
 
 extern "C" int64_t rmem_bank8_append_workspace(const rmem_bank8_append_args* a) {
@@ -424,19 +592,21 @@ extern "C" int rmem_bank8_append(const rmem_bank8_append_args* a, void* stream) 
     hipLaunchKernelGGL(mark_kernel, grid, dim3(256), 0, s, *a, marks, ps);
     RMEM_CHECK_LAUNCH();
   }
-  hipLaunchKernelGGL(append_kernel, dim3(a->rows, a->bank.heads, 2), dim3(256), 0, s, *a, marks, ps);
+  // rows of a workgroup: one while that leaves the chip room (a step of single tokens), up to 32 of a long call's, most of whose
+  // rows begin no page
+  const long groups = (long)a->rows * a->bank.heads * 2;
+  const int window = groups <= APPEND_GROUPS ? 1 : groups >= 32L * APPEND_GROUPS ? 32 : (int)((groups + APPEND_GROUPS - 1) / APPEND_GROUPS);
+  dispatch<Append>(a->type, a->bank.code, a->bank.dim, *a, marks, ps, window, s);
   RMEM_CHECK_LAUNCH();
   return RMEM_OK;
 }
 
 extern "C" int rmem_bank8_gather(const rmem_bank8_gather_args* a, void* stream) {
-  if (!a || !valid_bank(&a->bank) || !valid_type(a->type) || a->rows < 0) return RMEM_ERR_INVALID;
+  if (!a || !valid_bank(&a->bank) || !valid_type(a->type) || a->rows < 0 || a->bank.heads > 65535) return RMEM_ERR_INVALID;
   if (a->rows == 0) return RMEM_OK;
   if (!a->slots || !a->ko || !a->vo || ((uintptr_t)a->ko % 16) || ((uintptr_t)a->vo % 16)) return RMEM_ERR_INVALID;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const long units = (long)a->rows * a->bank.heads * (a->bank.dim / 16), blocks = (units + 255) / 256;
-  if (blocks >= 1 << 24) return RMEM_ERR_INVALID;
-  hipLaunchKernelGGL(gather_kernel, dim3((unsigned)blocks), dim3(256), 0, s, *a, log2_of(a->bank.page));
+  dispatch<Gather>(a->type, a->bank.code, a->bank.dim, *a, log2_of(a->bank.page), s);
   RMEM_CHECK_LAUNCH();
   return RMEM_OK;
 }
