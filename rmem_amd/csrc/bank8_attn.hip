@@ -67,14 +67,19 @@ __device__ __forceinline__ Req request(const rmem_bank8_attn_args& a, int r, con
   return x;
 }
 
-__device__ __forceinline__ long wave_sum_long(long v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) {
-    const unsigned lo = __shfl_xor((unsigned)v, o), hi = __shfl_xor((unsigned)((unsigned long)v >> 32), o);
-    v += (long)(((unsigned long)hi << 32) | lo);
-  }
+// Inclusive sums over the lanes in six DPP additions (shifts by 1, 2, 4, 8 within rows of 16, then the rows' last lanes): the same by
+// __shfl_up is six LDS round trips, and every workgroup begins with it.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);       // lane 15 of rows 0 and 2 to rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);       // lane 31 to rows 2 and 3
   return v;
 }
+// sum over the lanes; exact below 2^53, and the same everywhere
+__device__ __forceinline__ long wave_sum_long(long v) { return (long)wave_sum_xor_t<32>((double)v); }
 
 // tiles of a part
 template <int ROWS>
@@ -99,16 +104,7 @@ __device__ bool find_unit(const rmem_bank8_attn_args& a, const Split& sp, long i
     if (b) x = request<ROWS>(a, b + lane, sp);
     const int ns = x.tiles > chunk ? (x.tiles + chunk - 1) / chunk : 1;
     const int cnt = x.rt * ns, split = ns > 1 ? cnt : 0, ord = ns > 1 ? x.rt : 0;
-    int c = cnt, s = split, o = ord;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int cu = __shfl_up(c, d), su = __shfl_up(s, d), ou = __shfl_up(o, d);
-      if (lane >= d) {
-        c += cu;
-        s += su;
-        o += ou;
-      }
-    }
+    const int c = wave_scan(cnt), s = wave_scan(split), o = wave_scan(ord);
     const unsigned long long hit = __ballot(index < seen + c);
     if (hit) {
       const int l = __builtin_ctzll(hit);
@@ -374,10 +370,20 @@ __device__ __forceinline__ void attend_tiles(Acc<R, D>& c, const Query<R, D, NS>
 #pragma unroll
     for (int st = 0; st < N / 8; ++st) {
       frag8_t p, pl;
+      if constexpr (NS == 2) {
+        u32x4_t h, l;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        p[e] = (_Float16)s[i][8 * st + e];
-        if constexpr (NS == 2) pl[e] = (_Float16)(s[i][8 * st + e] - (float)p[e]);
+        for (int e = 0; e < 4; ++e) {
+          uint32_t hh, ll;
+          split_pair_f16(s[i][8 * st + 2 * e], s[i][8 * st + 2 * e + 1], hh, ll);
+          h[e] = hh;
+          l[e] = ll;
+        }
+        p = __builtin_bit_cast(frag8_t, h);
+        pl = __builtin_bit_cast(frag8_t, l);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = (_Float16)s[i][8 * st + e];
       }
 #pragma unroll
       for (int d = 0; d < D / R; ++d) {
