@@ -262,9 +262,9 @@ __device__ __forceinline__ const T* element(const T* src, long ldr, int r, int a
 // them) leaves too few workgroups to hide the chain slots -> rows -> maximum -> codes.  Keys: a thread takes 16 dims of a token,
 // eight threads a token of 128 dims (256 bytes in, 128-byte pieces out).  Values: a thread takes 16 tokens (half a 32-token tile)
 // of two dims, so that a wave reads whole rows and each thread writes the two chunks that hold its tokens.
-template <class T, int CODE, int D, bool FAST>
-__global__ __launch_bounds__(256, 4) void append_kernel(rmem_bank8_append_args a, const PageMark* marks, int ps, int window) {
-  __shared__ float s_max[4];
+template <class T, int CODE, int D, bool FAST, int NT>
+__global__ __launch_bounds__(NT, 4) void append_kernel(rmem_bank8_append_args a, const PageMark* marks, int ps, int window) {
+  __shared__ float s_max[NT / 64];
   __shared__ __attribute__((aligned(16))) int s_row[128];   // row that fills each place of the page, -1: none; the last of several
   __shared__ int s_other;
   const int h = blockIdx.y, part = blockIdx.z;
@@ -295,14 +295,16 @@ __global__ __launch_bounds__(256, 4) void append_kernel(rmem_bank8_append_args a
     __syncthreads();                      // the page before has been written
     if (runs == 1) {
       // the run goes on where the slots do; a row further on that fitted the pattern again would begin another run
-      const long r = (long)row + tid - off;
-      if (tid < 128) s_row[tid] = tid >= off && tid < page && r < a.rows && a.slots[r] == slot + tid - off ? (int)r : -1;
+      for (int i = tid; i < 128; i += NT) {
+        const long r = (long)row + i - off;
+        s_row[i] = i >= off && i < page && r < a.rows && a.slots[r] == slot + i - off ? (int)r : -1;
+      }
       if (tid == 0) s_other = 0;
     } else {
-      if (tid < 128) s_row[tid] = -1;
+      for (int i = tid; i < 128; i += NT) s_row[i] = -1;
       if (tid == 0) s_other = 0;
       __syncthreads();
-      for (int r = marks ? row + tid : tid; r < a.rows; r += 256) {
+      for (int r = marks ? row + tid : tid; r < a.rows; r += NT) {
         const int s = a.slots[r];
         if (s < 0 || (s >> ps) != pg32) continue;
         if (r < row) s_other = 1;
@@ -320,12 +322,12 @@ __global__ __launch_bounds__(256, 4) void append_kernel(rmem_bank8_append_args a
     // the new tokens' largest value, four loads of eight elements in flight per thread
     float mx = 0.f;
     constexpr int W = D / 8;
-    for (int u0 = tid; u0 < (hi - lo) * W; u0 += 4 * 256) {
+    for (int u0 = tid; u0 < (hi - lo) * W; u0 += 4 * NT) {
       Run<T, 8, FAST> y[4];
       int r[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int u = u0 + i * 256, place = lo + u / W;
+        const int u = u0 + i * NT, place = lo + u / W;
         r[i] = place < hi ? s_row[place] : -1;
         y[i].load(element<T, FAST>(src, ldr, r[i] < 0 ? row : r[i], (u % W) * 8));
       }
@@ -337,7 +339,8 @@ __global__ __launch_bounds__(256, 4) void append_kernel(rmem_bank8_append_args a
     mx = wave_max_xor(mx);
     if (lane == 0) s_max[wave] = mx;
     __syncthreads();
-    mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) mx = fmaxf(mx, s_max[w]);
     const float was = lo ? before : 0.f, fresh = fmaxf(mx, 1e-30f) / (CODE == INT8 ? 127.f : 448.f);
     const bool grown = lo && fresh > was;
     const float scale = lo && !grown ? was : fresh;
@@ -349,18 +352,18 @@ __global__ __launch_bounds__(256, 4) void append_kernel(rmem_bank8_append_args a
     if (!part) {
       constexpr int C = D / 16;
       auto at = [&](int key, int c) { return reinterpret_cast<u32x4_t*>(codes + ((long)c * page + key) * 16); };
-      for (int u0 = tid; u0 < (hi - lo) * C; u0 += 2 * 256) {
+      for (int u0 = tid; u0 < (hi - lo) * C; u0 += 2 * NT) {
         Run<T, 16, FAST> y[2];
         int r[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int u = u0 + i * 256, key = lo + u / C;
+          const int u = u0 + i * NT, key = lo + u / C;
           r[i] = key < hi ? s_row[key] : -1;
           y[i].load(element<T, FAST>(src, ldr, r[i] < 0 ? row : r[i], (u % C) * 16));
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int u = u0 + i * 256;
+          const int u = u0 + i * NT;
           if (r[i] < 0) continue;
           u32x4_t w;
 #pragma unroll
@@ -370,7 +373,7 @@ __global__ __launch_bounds__(256, 4) void append_kernel(rmem_bank8_append_args a
         }
       }
       if (grown || (holes && !lo))
-        for (int u = tid; u < hi * C; u += 256) {
+        for (int u = tid; u < hi * C; u += NT) {
           const int key = u / C;
           if (s_row[key] >= 0) continue;
           u32x4_t w = *at(key, u % C);
@@ -382,7 +385,7 @@ __global__ __launch_bounds__(256, 4) void append_kernel(rmem_bank8_append_args a
       constexpr int P = D / 2;
       const int t0 = lo >> 5, t1 = (hi + 31) >> 5;
       auto at = [&](int th, int d) { return reinterpret_cast<u32x4_t*>(codes + ((long)th * D + d) * 16); };
-      for (int u = 2 * t0 * P + tid; u < 2 * t1 * P; u += 256) {
+      for (int u = 2 * t0 * P + tid; u < 2 * t1 * P; u += NT) {
         const int th = u / P, d = 2 * (u % P);
         Run<T, 2, FAST> y[16];
         uint32_t fill[4];
@@ -415,7 +418,7 @@ __global__ __launch_bounds__(256, 4) void append_kernel(rmem_bank8_append_args a
         *at(th, d + 1) = w[1];
       }
       if (grown)
-        for (int u = tid; u < 2 * t0 * D; u += 256) {
+        for (int u = tid; u < 2 * t0 * D; u += NT) {
           u32x4_t w = *at(u / D, u % D);
 #pragma unroll
           for (int e = 0; e < 4; ++e) w[e] = recode4<CODE>(w[e], ratio);
@@ -535,8 +538,11 @@ struct Append {
     const unsigned long mis = (unsigned long)a.k | (unsigned long)a.v | (unsigned long)((a.k_row | a.k_head | a.v_row | a.v_head) * (long)sizeof(T));
     const dim3 grid((a.rows + window - 1) / window, a.bank.heads, 2);
     const long span = (a.rows - 1L) * std::max(a.k_row, a.v_row) + D;
-    if ((mis & 15) || span * (long)sizeof(T) >= 1L << 32) hipLaunchKernelGGL((append_kernel<T, CODE, D, false>), grid, dim3(256), 0, s, a, marks, ps, window);
-    else hipLaunchKernelGGL((append_kernel<T, CODE, D, true>), grid, dim3(256), 0, s, a, marks, ps, window);
+    // Up to SCAN_ROWS rows most pages get a token or a few: workgroups of 128 keep more of their chains of reads in flight (1000
+    // single tokens: 47 us, 65 with 256); long calls fill whole pages, which 256 write faster (25 k tokens into pages of 128: 47, 56).
+    if ((mis & 15) || span * (long)sizeof(T) >= 1L << 32) hipLaunchKernelGGL((append_kernel<T, CODE, D, false, 128>), grid, dim3(128), 0, s, a, marks, ps, window);
+    else if (!marks) hipLaunchKernelGGL((append_kernel<T, CODE, D, true, 128>), grid, dim3(128), 0, s, a, marks, ps, window);
+    else hipLaunchKernelGGL((append_kernel<T, CODE, D, true, 256>), grid, dim3(256), 0, s, a, marks, ps, window);
   }
 };
 template <class T, int CODE, int D>
@@ -592,10 +598,10 @@ extern "C" int rmem_bank8_append(const rmem_bank8_append_args* a, void* stream) 
     hipLaunchKernelGGL(mark_kernel, grid, dim3(256), 0, s, *a, marks, ps);
     RMEM_CHECK_LAUNCH();
   }
-  // rows of a workgroup: one while that leaves the chip room (a step of single tokens), up to 32 of a long call's, most of whose
-  // rows begin no page
+  // rows of a workgroup: one while that leaves the chip room (a step of single tokens), up to 64 of a long call's, most of whose
+  // rows begin no page (25 k rows of prompts: 63 us with up to 32, 52 us with up to 64)
   const long groups = (long)a->rows * a->bank.heads * 2;
-  const int window = groups <= APPEND_GROUPS ? 1 : groups >= 32L * APPEND_GROUPS ? 32 : (int)((groups + APPEND_GROUPS - 1) / APPEND_GROUPS);
+  const int window = groups <= APPEND_GROUPS ? 1 : groups >= 64L * APPEND_GROUPS ? 64 : (int)((groups + APPEND_GROUPS - 1) / APPEND_GROUPS);
   dispatch<Append>(a->type, a->bank.code, a->bank.dim, *a, marks, ps, window, s);
   RMEM_CHECK_LAUNCH();
   return RMEM_OK;
