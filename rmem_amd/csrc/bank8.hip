@@ -608,7 +608,7 @@ extern "C" int rmem_bank8_append(const rmem_bank8_append_args* a, void* stream) 
 }
 
 extern "C" int rmem_bank8_gather(const rmem_bank8_gather_args* a, void* stream) {
-  if (!a || !valid_bank(&a->bank) || !valid_type(a->type) || a->rows < 0 || a->bank.heads > 65535) return RMEM_ERR_INVALID;
+  if (!a || !valid_bank(&a->bank) || !valid_type(a->type) || a->rows < 0 || a->rows >= 1 << 30 || a->bank.heads > 65535) return RMEM_ERR_INVALID;
   if (a->rows == 0) return RMEM_OK;
   if (!a->slots || !a->ko || !a->vo || ((uintptr_t)a->ko % 16) || ((uintptr_t)a->vo % 16)) return RMEM_ERR_INVALID;
   hipStream_t s = static_cast<hipStream_t>(stream);

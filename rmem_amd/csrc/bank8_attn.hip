@@ -32,7 +32,7 @@ constexpr float VS_MIN = 3.23117427e-27f;    // 2^-88: 1 / vs times 2^15 times 2
 // A unit of work is (request, tile of ROWS rows, one of ns equal parts of the tokens that the tile sees) for one kv head.  Every
 // part has at most `chunk` 32-token tiles, chunk = (all row tiles' token tiles) / want, so the parts of long and short requests
 // cost the same and nothing is decided on the host, which does not know the lengths.  Each wave computes the same division from
-// cu and lens: 64 requests at a time, two passes (total, then position).
+// cu and lens, a request per lane.
 struct Unit {
   int r, rt, part, ns;    // request, row tile, part of ns
   int q0, n, len;         // first row, rows, tokens
@@ -81,64 +81,129 @@ __device__ __forceinline__ int wave_scan(int v) {
 // sum over the lanes; exact below 2^53, and the same everywhere
 __device__ __forceinline__ long wave_sum_long(long v) { return (long)wave_sum_xor_t<32>((double)v); }
 
-// tiles of a part
-template <int ROWS>
-__device__ __forceinline__ int chunk_of(const rmem_bank8_attn_args& a, const Split& sp, const Req& first) {
-  const int lane = threadIdx.x & 63;
-  long total = (long)first.rt * first.tiles;
-  for (int b = 64; b < a.reqs; b += 64) {
-    const Req y = request<ROWS>(a, b + lane, sp);
-    total += (long)y.rt * y.tiles;
-  }
-  total = (wave_sum_long(total) + sp.want - 1) / sp.want;
+// tiles of a part (up to 64 requests, one per lane)
+__device__ __forceinline__ int chunk_of(const Req& x, const Split& sp) {
+  const long total = (wave_sum_long((long)x.rt * x.tiles) + sp.want - 1) / sp.want;
   return total < sp.chunk_min ? sp.chunk_min : total > 0x3fffffff ? 0x3fffffff : (int)total;
 }
 
+// With more requests than lanes the division is computed once, by a launch of its own (index_kernel), and looked up: what lies in
+// front of each request, and last the totals.  (Requests of one row and up to 1000 tokens, 64 at a time scanned by every workgroup:
+// 1000 of them 280 us, looked up 175 us; 200 of them 100 and 98.)
+struct Before {
+  int units, slots, ords, chunk;
+};
+
 template <int ROWS>
-__device__ bool find_unit(const rmem_bank8_attn_args& a, const Split& sp, long index, Unit& u) {
+__device__ __forceinline__ bool look_up(const rmem_bank8_attn_args& a, const Split& sp, const Before* index, long at, Unit& u) {
   const int lane = threadIdx.x & 63;
-  Req x = request<ROWS>(a, lane, sp);
-  const int chunk = chunk_of<ROWS>(a, sp, x);
-  long seen = 0, slots = 0, ords = 0;
-  for (int b = 0; b < a.reqs; b += 64) {
-    if (b) x = request<ROWS>(a, b + lane, sp);
-    const int ns = x.tiles > chunk ? (x.tiles + chunk - 1) / chunk : 1;
-    const int cnt = x.rt * ns, split = ns > 1 ? cnt : 0, ord = ns > 1 ? x.rt : 0;
-    const int c = wave_scan(cnt), s = wave_scan(split), o = wave_scan(ord);
-    const unsigned long long hit = __ballot(index < seen + c);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      u.ns = __builtin_amdgcn_readlane(ns, l);
-      const int k = (int)(index - seen) - (__builtin_amdgcn_readlane(c, l) - __builtin_amdgcn_readlane(cnt, l));
-      u.r = b + l;
-      u.rt = __builtin_amdgcn_readlane(x.rt, l) - 1 - k / u.ns;      // the last row tile first: under a causal mask it sees most
-      u.part = k % u.ns;
-      u.q0 = __builtin_amdgcn_readlane(x.q0, l);
-      u.n = __builtin_amdgcn_readlane(x.n, l);
-      u.len = __builtin_amdgcn_readlane(x.len, l);
-      u.slot = (int)slots + __builtin_amdgcn_readlane(s, l) - __builtin_amdgcn_readlane(split, l) + u.rt * u.ns;
-      u.ord = (int)ords + __builtin_amdgcn_readlane(o, l) - __builtin_amdgcn_readlane(ord, l) + u.rt;
-      return true;
-    }
-    seen += __builtin_amdgcn_readlane(c, 63);
-    slots += __builtin_amdgcn_readlane(s, 63);
-    ords += __builtin_amdgcn_readlane(o, 63);
+  if (at >= index[a.reqs].units) return false;
+  int lo = 0, len = a.reqs;                    // the last request with no more than `at` units in front of it, 64 places at a time
+  while (len > 1) {
+    const int step = (len + 63) >> 6, r = lo + lane * step;
+    const bool le = lane * step < len && index[r].units <= at;
+    const int n = __popcll(__ballot(le));
+    lo += (n - 1) * step;
+    len = min(step, len - (n - 1) * step);
   }
-  return false;
+  const Before b = index[lo];
+  const Req x = request<ROWS>(a, lo, sp);
+  const int k = (int)(at - b.units);
+  u.ns = x.tiles > b.chunk ? (x.tiles + b.chunk - 1) / b.chunk : 1;
+  u.r = lo;
+  u.rt = x.rt - 1 - k / u.ns;
+  u.part = k % u.ns;
+  u.q0 = x.q0;
+  u.n = x.n;
+  u.len = x.len;
+  u.slot = b.slots + u.rt * u.ns;
+  u.ord = b.ords + u.rt;
+  return u.rt >= 0;
+}
+
+template <int ROWS>
+__global__ __launch_bounds__(1024) void index_kernel(rmem_bank8_attn_args a, Split sp, Before* index) {
+  __shared__ double s_sum[16];
+  __shared__ int s_part[3][16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  double total = 0;
+  for (int r = tid; r < a.reqs; r += 1024) {
+    const Req x = request<ROWS>(a, r, sp);
+    total += (double)x.rt * x.tiles;
+  }
+  total = wave_sum_xor_t<32>(total);
+  if (lane == 0) s_sum[wave] = total;
+  __syncthreads();
+  total = 0;
+  for (int w = 0; w < 16; ++w) total += s_sum[w];
+  const long even = ((long)total + sp.want - 1) / sp.want;
+  const int chunk = even < sp.chunk_min ? sp.chunk_min : even > 0x3fffffff ? 0x3fffffff : (int)even;
+  int seen[3] = {0, 0, 0};
+  for (int base = 0; base < a.reqs; base += 1024) {
+    const Req x = request<ROWS>(a, base + tid, sp);
+    const int ns = x.tiles > chunk ? (x.tiles + chunk - 1) / chunk : 1;
+    const int own[3] = {x.rt * ns, ns > 1 ? x.rt * ns : 0, ns > 1 ? x.rt : 0};
+    int sum[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      sum[i] = wave_scan(own[i]);
+      if (lane == 63) s_part[i][wave] = sum[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      int front = seen[i];
+      for (int w = 0; w < 16; ++w) {
+        const int p = s_part[i][w];
+        if (w < wave) front += p;
+        seen[i] += p;
+      }
+      sum[i] += front - own[i];
+    }
+    if (base + tid < a.reqs) {
+      const Before b = {sum[0], sum[1], sum[2], chunk};
+      index[base + tid] = b;
+    }
+    __syncthreads();
+  }
+  if (tid == 0) {
+    const Before b = {seen[0], seen[1], seen[2], chunk};
+    index[a.reqs] = b;
+  }
+}
+
+template <int ROWS>
+__device__ bool find_unit(const rmem_bank8_attn_args& a, const Split& sp, const Before* before, long index, Unit& u) {
+  if (before) return look_up<ROWS>(a, sp, before, index, u);
+  const int lane = threadIdx.x & 63;
+  const Req x = request<ROWS>(a, lane, sp);
+  const int chunk = chunk_of(x, sp);
+  const int ns = x.tiles > chunk ? (x.tiles + chunk - 1) / chunk : 1;
+  const int cnt = x.rt * ns, split = ns > 1 ? cnt : 0, ord = ns > 1 ? x.rt : 0;
+  const int c = wave_scan(cnt), s = wave_scan(split), o = wave_scan(ord);
+  const unsigned long long hit = __ballot(index < c);
+  if (!hit) return false;
+  const int l = __builtin_ctzll(hit);
+  u.ns = __builtin_amdgcn_readlane(ns, l);
+  const int k = (int)index - (__builtin_amdgcn_readlane(c, l) - __builtin_amdgcn_readlane(cnt, l));
+  u.r = l;
+  u.rt = __builtin_amdgcn_readlane(x.rt, l) - 1 - k / u.ns;      // the last row tile first: under a causal mask it sees most
+  u.part = k % u.ns;
+  u.q0 = __builtin_amdgcn_readlane(x.q0, l);
+  u.n = __builtin_amdgcn_readlane(x.n, l);
+  u.len = __builtin_amdgcn_readlane(x.len, l);
+  u.slot = __builtin_amdgcn_readlane(s, l) - __builtin_amdgcn_readlane(split, l) + u.rt * u.ns;
+  u.ord = __builtin_amdgcn_readlane(o, l) - __builtin_amdgcn_readlane(ord, l) + u.rt;
+  return true;
 }
 
 // row tiles in several parts
 template <int ROWS>
-__device__ __forceinline__ long count_split(const rmem_bank8_attn_args& a, const Split& sp) {
-  const int lane = threadIdx.x & 63;
-  Req x = request<ROWS>(a, lane, sp);
-  const int chunk = chunk_of<ROWS>(a, sp, x);
-  long n = 0;
-  for (int b = 0; b < a.reqs; b += 64) {
-    if (b) x = request<ROWS>(a, b + lane, sp);
-    if (x.tiles > chunk) n += x.rt;
-  }
-  return wave_sum_long(n);
+__device__ __forceinline__ long count_split(const rmem_bank8_attn_args& a, const Split& sp, const Before* before) {
+  if (before) return before[a.reqs].ords;
+  const Req x = request<ROWS>(a, threadIdx.x & 63, sp);
+  const int chunk = chunk_of(x, sp);
+  return wave_sum_long(x.tiles > chunk ? x.rt : 0);
 }
 
 // ---------------------------------------------------------------------------------------------------------- one token tile
@@ -451,6 +516,7 @@ struct Parts {
   float* o;
   float* ml;
   Split_tile* tiles;
+  const Before* before;   // the division, looked up (null: computed)
   int slots, ords;        // units and tiles that fit
 };
 
@@ -565,7 +631,7 @@ __global__ __launch_bounds__(256, 2) void attn_narrow(rmem_bank8_attn_args a, Pa
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);       // uniform: tile counts and page addresses stay scalar
   const int heads = a.bank.heads, h = blockIdx.x % heads;
   Unit u;
-  if (!find_unit<R>(a, sp, blockIdx.x / heads, u)) return;
+  if (!find_unit<R>(a, sp, parts.before, blockIdx.x / heads, u)) return;
   const int row = u.rt * R + j, qt = row / G, hq = h * G + row % G;
   const bool on = qt < u.n;
   const int lim = !on ? 0 : a.causal ? min(u.len, u.len - u.n + qt + 1) : u.len;     // may be <= 0
@@ -680,7 +746,7 @@ __global__ __launch_bounds__(256, NS == 2 && D == 128 ? 1 : 2) void attn_wide(rm
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int heads = a.bank.heads, h = blockIdx.x % heads;
   Unit u;
-  if (!find_unit<WROWS>(a, sp, blockIdx.x / heads, u)) return;
+  if (!find_unit<WROWS>(a, sp, parts.before, blockIdx.x / heads, u)) return;
   const int row0 = u.rt * WROWS + wave * R, row = row0 + j, qt = row / G, hq = h * G + row % G;
   const bool on = qt < u.n;
   const int lim = !on ? 0 : a.causal ? min(u.len, u.len - u.n + qt + 1) : u.len;
@@ -821,7 +887,7 @@ __global__ __launch_bounds__(256) void attn_merge(rmem_bank8_attn_args a, Parts 
   const int heads = a.bank.heads, lane = threadIdx.x & 63, G = sp.G;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool wide = wide_stores(a);
-  const long tiles = count_split<ROWS>(a, sp), items = (tiles < parts.ords ? tiles : parts.ords) * heads * BLOCKS;
+  const long tiles = count_split<ROWS>(a, sp, parts.before), items = (tiles < parts.ords ? tiles : parts.ords) * heads * BLOCKS;
   auto finish = [&](const Split_tile& t, int h, int j, int d4, f32x4_t o, float m, float l, bool mine) __attribute__((always_inline)) {
     const int row = t.rt * ROWS + j, hq = h * G + row % G;
     const long at = t.q0 + row / G;
@@ -835,7 +901,10 @@ __global__ __launch_bounds__(256) void attn_merge(rmem_bank8_attn_args a, Parts 
     const long th = item / BLOCKS;
     const int h = (int)(th % heads), end = (int)(item % BLOCKS + 1) * BLOCK;
     const Split_tile t = parts.tiles[th / heads];
-    if (t.slot + t.ns > parts.slots) continue;
+    // (row offsets that are none -- requests that overlap -- can leave a descriptor unwritten)
+    if (t.slot < 0 || t.ns < 2 || t.ns > parts.slots - t.slot || t.q0 < 0 || t.n < 0 || t.n > a.rows - t.q0 || t.rt < 0 ||
+        t.rt > 0x7fffffff / ROWS - 1)
+      continue;
     const int rows = min(end, t.n * G - t.rt * ROWS);        // of the tile that exist (n * G < 2^31: checked on the host)
     const long step = (long)heads * ROWS;
     if (t.ns <= FEW_PARTS) {
@@ -890,15 +959,17 @@ __global__ __launch_bounds__(256) void attn_merge(rmem_bank8_attn_args a, Parts 
 }
 
 // -------------------------------------------------------------------------------------------------------------------- host
-#ifndef NL
-#define NL 256
-#endif
 constexpr int ROWS16 = 16;              // requests of at most this many rows per kv head take tiles of 16 rows
-constexpr int NARROW_ROWS = NL;         // up to this many the narrow kernel, beyond the wide one
+// Up to this many the narrow kernel, beyond the wide one.  4 requests of 256 rows over 16 k tokens of 128 dims: narrow 61 us, wide 72;
+// of 256 single-head rows over 8 k tokens of 64 dims: 44 and 67; 512 causal rows over 64 k tokens: the wide kernel, 820 TFLOP/s.
+constexpr int NARROW_ROWS = 256;
 constexpr int NARROW_CHUNK = 8;         // fewest 32-token tiles worth a part
 constexpr int WIDE_CHUNK = 16;
 
-// parts of all kv heads that a read is divided into: as many as workgroups fit the chip at once
+// Parts of all kv heads that a read is divided into.  Narrow: as many as workgroups fit the chip at once (registers), which a larger
+// number only adds starts and parts to merge to (64 ragged requests of 128 dims: 512 parts 100 us, 1024 101, 2048 104; of 32 dims 1536
+// parts 33, 512 39).  Wide: the same at 128 dims (512 rows over 64 k tokens: 512 parts 674 us, 2048 748); smaller dims have shorter
+// units, which even out what a causal mask makes uneven (4 x 2000 causal rows of 64 dims: 2048 parts 164, 512 185).
 int narrow_units(int dim) { return dim == 128 ? 512 : dim == 64 ? 1024 : 1536; }
 int wide_units(int dim) { return dim == 128 ? 512 : 2048; }
 
@@ -916,7 +987,7 @@ bool valid_attn(const rmem_bank8_attn_args* a) {
       (int64_t)a->cols * a->bank.page > 0x7fffffff || a->heads_q <= 0 || a->heads_q % a->bank.heads || !(a->scale > 0.f) ||
       !(a->scale < 3.0e38f))
     return false;
-  return (int64_t)a->rows * (a->heads_q / a->bank.heads) <= 0x7fffffff;
+  return (int64_t)a->rows * (a->heads_q / a->bank.heads) <= 0x7fffff00;
 }
 
 Launch make_launch(const rmem_bank8_attn_args* a, int rows, int units, int chunk_min, int lo, int hi) {
@@ -933,7 +1004,8 @@ Launch make_launch(const rmem_bank8_attn_args* a, int rows, int units, int chunk
   l.tiles = std::min(l.tiles, reqs * (((long)hi + rows - 1) / rows));
   // parts: at most total / chunk + one per row tile; of requests in several parts, at most twice total / chunk
   l.units = l.sp.want + l.tiles;
-  l.slots = 2L * l.sp.want;
+  // a request whose row of the table holds no more than the smallest part is never divided
+  l.slots = ((long)a->cols * a->bank.page + 31) / 32 > chunk_min ? 2L * l.sp.want : 0;
   return l;
 }
 
@@ -950,9 +1022,11 @@ Plan make_plan(const rmem_bank8_attn_args* a) {
   return p;
 }
 
-// floats of a launch's workspace: partial results, references and sums, tiles in several parts (at most `want`: two parts each)
+// floats of a launch's workspace: partial results, references and sums, tiles in several parts (at most `want`: two parts each),
+// the division's index; each a multiple of 16 bytes
 long part_floats(const rmem_bank8_attn_args* a, const Launch& l) {
-  return l.slots * a->bank.heads * l.rows * (a->bank.dim + 2) + l.sp.want * (long)(sizeof(Split_tile) / 4);
+  const long index = a->reqs > 64 ? (a->reqs + 1L) * (long)(sizeof(Before) / 4) : 0;
+  return l.slots * a->bank.heads * l.rows * (a->bank.dim + 2) + (l.slots ? l.sp.want : 0) * (long)(sizeof(Split_tile) / 4) + index;
 }
 
 template <int D, int CODE, int NS>
@@ -969,8 +1043,7 @@ int launch_dim(const rmem_bank8_attn_args& a, const Parts& parts, const Launch& 
   if (e4m3) two ? launch_attn<D, E4M3, 2>(a, parts, l, s) : launch_attn<D, E4M3, 1>(a, parts, l, s);
   else two ? launch_attn<D, INT8, 2>(a, parts, l, s) : launch_attn<D, INT8, 1>(a, parts, l, s);
   RMEM_CHECK_LAUNCH();
-  // a request whose row of the table holds no more than the smallest part is never divided
-  if (((long)a.cols * a.bank.page + 31) / 32 > l.sp.chunk_min) {
+  if (l.slots) {
     const long tiles = l.tiles < l.sp.want ? l.tiles : l.sp.want;       // row tiles in at least two parts: at most `want`
     const dim3 grid((unsigned)std::min(tiles * a.bank.heads * (l.rows / merge_block(l.rows)), 2048L));
     if (l.rows == 16) hipLaunchKernelGGL((attn_merge<16, D>), grid, dim3(256), 0, s, a, parts, l.sp);
@@ -987,7 +1060,16 @@ int launch_read(const rmem_bank8_attn_args& a, float* ws, const Launch& l, hipSt
   parts.ml = ws + l.slots * a.bank.heads * l.rows * a.bank.dim;
   parts.tiles = reinterpret_cast<Split_tile*>(parts.ml + l.slots * a.bank.heads * l.rows * 2);
   parts.slots = (int)l.slots;
-  parts.ords = l.sp.want;
+  parts.ords = l.slots ? l.sp.want : 0;
+  parts.before = nullptr;
+  if (a.reqs > 64) {
+    Before* index = reinterpret_cast<Before*>(parts.tiles + parts.ords);
+    if (l.rows == 16) hipLaunchKernelGGL(index_kernel<16>, dim3(1), dim3(1024), 0, s, a, l.sp, index);
+    else if (l.rows == 32) hipLaunchKernelGGL(index_kernel<32>, dim3(1), dim3(1024), 0, s, a, l.sp, index);
+    else hipLaunchKernelGGL(index_kernel<WROWS>, dim3(1), dim3(1024), 0, s, a, l.sp, index);
+    RMEM_CHECK_LAUNCH();
+    parts.before = index;
+  }
   return a.bank.dim == 32 ? launch_dim<32>(a, parts, l, s) : a.bank.dim == 64 ? launch_dim<64>(a, parts, l, s) : launch_dim<128>(a, parts, l, s);
 }
 
@@ -1003,8 +1085,9 @@ extern "C" int rmem_bank8_attn(const rmem_bank8_attn_args* a, void* stream) {
   if (!valid_attn(a)) return RMEM_ERR_INVALID;
   if (a->rows == 0) return RMEM_OK;
   const Plan p = make_plan(a);
-  if (!a->q || !a->out || !a->cu || !a->lens || !a->table || !a->workspace || ((uintptr_t)a->workspace % 16) ||
-      a->workspace_bytes < rmem_bank8_attn_workspace(a) || p.narrow.units * a->bank.heads >= 1 << 24 || p.wide.units * a->bank.heads >= 1 << 24)
+  const int64_t need = rmem_bank8_attn_workspace(a);
+  if (!a->q || !a->out || !a->cu || !a->lens || !a->table ||
+      (need && (!a->workspace || ((uintptr_t)a->workspace % 16) || a->workspace_bytes < need)) || p.narrow.units * a->bank.heads >= 1 << 24 || p.wide.units * a->bank.heads >= 1 << 24)
     return RMEM_ERR_INVALID;
   hipStream_t s = static_cast<hipStream_t>(stream);
   float* ws = static_cast<float*>(a->workspace);

@@ -90,11 +90,10 @@ class PlainPool:
     def values(self, w):
         return decode(self.codes[w], self.code) * self.scale[w].astype(np.float64)[:, None, :, None]
 
-    def tokens(self, w, table_row, length):
-        """[length, heads, dim] of a request"""
-        v = self.values(w)
-        return np.stack([v[table_row[t // self.page], t % self.page] for t in range(length)]) if length else \
-            np.zeros((0, self.heads, self.dim))
+    def tokens(self, values, table_row, length):
+        """[length, heads, dim] of a request, from values(w)"""
+        t = np.arange(length)
+        return values[np.asarray(table_row)[t // self.page], t % self.page]
 
     def to_device(self, B):
         p = B.Pool.empty(self.pages, self.heads, self.dim, self.page, self.code, DEV)
@@ -165,9 +164,10 @@ def attend64(pool, q, cu, lens, table, causal, scale):
     out, mean = np.zeros((rows, hq, dim)), np.zeros((rows, hq, dim))
     lse, most = np.full((rows, hq), -np.inf), np.zeros((rows, hq))
     group = hq // pool.heads
+    all_k, all_v = pool.values("k"), pool.values("v")
     for r in range(len(lens)):
         ln, n = int(lens[r]), int(cu[r + 1] - cu[r])
-        k, v = pool.tokens("k", table[r], ln), pool.tokens("v", table[r], ln)
+        k, v = pool.tokens(all_k, table[r], ln), pool.tokens(all_v, table[r], ln)
         for i in range(n):
             sees = min(ln, ln - n + i + 1) if causal else ln
             if sees <= 0:
@@ -290,7 +290,7 @@ def test_c_abi_refuses_bad_arguments():
             setattr(a, n, val)
         assert lib.rmem_bank8_gather(C.byref(a), None) == -1, bad
     good = dict(bank=b, q=_addr(4), out=_addr(5), lse=0, type=1, q_row=256, q_head=64, o_row=256, o_head=64, cu=_addr(6), lens=_addr(7),
-                reqs=2, rows=4, table=_addr(8), ld_table=4, cols=4, heads_q=4, max_rows=2, causal=1, scale=0.125, workspace=_addr(20),
+                reqs=2, rows=4, table=_addr(8), ld_table=16, cols=16, heads_q=4, max_rows=2, causal=1, scale=0.125, workspace=_addr(20),
                 workspace_bytes=1 << 40)
     for bad in (dict(q=0), dict(out=0), dict(cu=0), dict(lens=0), dict(table=0), dict(workspace=0), dict(workspace=_addr(20) + 4),
                 dict(workspace_bytes=16), dict(type=3), dict(reqs=0), dict(rows=-1), dict(cols=0), dict(ld_table=3), dict(heads_q=3),
@@ -333,7 +333,7 @@ def test_python_refuses_mismatched_device_tensors(B):
                 (k.to(torch.float64), k.to(torch.float64), i(4))):
         with pytest.raises(RmemError):
             B.append(pool, *bad)
-    q, cu, lens, table = f(3, 4, 64), i(3), i(2), i(2, 4)
+    q, cu, lens, table = f(3, 4, 64), i(3), i(2), i(2, 16)
     B.attend(pool, q, cu, lens, table)
     for kw in (dict(q=f(3, 3, 64)), dict(q=f(3, 4, 32)), dict(cu=i(2)), dict(lens=i(2, dt=torch.int64)), dict(table=i(3, 4)),
                dict(table=i(2, 0)), dict(table=i(4, 2).t()), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
@@ -659,7 +659,7 @@ def test_attend_groups(B, group):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("reqs", [63, 64, 65, 130])
+@pytest.mark.parametrize("reqs", [63, 64, 65, 130, 1100, 4200])
 def test_attend_many_requests(B, reqs):
     rs = np.random.RandomState(reqs)
     lens = rs.randint(0, 90, reqs)
