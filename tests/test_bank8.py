@@ -168,19 +168,21 @@ def attend64(pool, q, cu, lens, table, causal, scale):
     for r in range(len(lens)):
         ln, n = int(lens[r]), int(cu[r + 1] - cu[r])
         k, v = pool.tokens(all_k, table[r], ln), pool.tokens(all_v, table[r], ln)
-        for i in range(n):
-            sees = min(ln, ln - n + i + 1) if causal else ln
-            if sees <= 0:
-                continue
-            for h in range(hq):
-                qq, kk, vv = q[cu[r] + i, h], k[:sees, h // group], v[:sees, h // group]
-                s = kk @ qq * scale
-                m = s.max()
-                p = np.exp(s - m)
-                out[cu[r] + i, h] = p @ vv / p.sum()
-                mean[cu[r] + i, h] = p @ np.abs(vv) / p.sum()
-                lse[cu[r] + i, h] = m + math.log(p.sum())
-                most[cu[r] + i, h] = (np.abs(kk) @ np.abs(qq)).max() * scale
+        if not n or not ln:
+            continue
+        rows = slice(int(cu[r]), int(cu[r]) + n)
+        sees = np.arange(ln)[None] < (ln - n + np.arange(n) + 1 if causal else np.full(n, ln))[:, None]
+        on = sees.any(1)
+        for h in range(hq):
+            qq, kk, vv = q[rows, h], k[:, h // group], v[:, h // group]
+            s = np.where(sees, qq @ kk.T * scale, -np.inf)
+            m = np.where(on, s.max(1), 0.0)
+            p = np.exp(s - m[:, None])
+            total = np.where(on, p.sum(1), 1.0)
+            out[rows, h] = p @ vv / total[:, None]
+            mean[rows, h] = p @ np.abs(vv) / total[:, None]
+            lse[rows, h] = np.where(on, m + np.log(total), -np.inf)
+            most[rows, h] = np.where(sees, np.abs(qq) @ np.abs(kk).T, 0.0).max(1) * scale
     return out, lse, mean, most
 
 
@@ -337,7 +339,7 @@ def test_python_refuses_mismatched_device_tensors(B):
     B.attend(pool, q, cu, lens, table)
     for kw in (dict(q=f(3, 3, 64)), dict(q=f(3, 4, 32)), dict(cu=i(2)), dict(lens=i(2, dt=torch.int64)), dict(table=i(3, 4)),
                dict(table=i(2, 0)), dict(table=i(4, 2).t()), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
-               dict(out=f(3, 4, 64, dt=torch.float32)), dict(out=f(2, 4, 64)), dict(lse=f(3, 4)), dict(workspace=f(4, dt=torch.uint8))):
+               dict(out=f(3, 4, 64, dt=torch.float32)), dict(out=f(2, 4, 64)), dict(out=f(1, 4, 64).expand(3, 4, 64)), dict(lse=f(3, 4)), dict(workspace=f(4, dt=torch.uint8))):
         a = dict(pool=pool, q=q, cu=cu, lens=lens, table=table)
         a.update(kw)
         with pytest.raises(RmemError):
@@ -644,6 +646,126 @@ def test_attend(B, code, kind, case, page, heads, group, dim):
     cu = np.concatenate([[0], np.cumsum(n)])
     q = dense(rs, int(cu[-1]), heads * group, dim, kind, 0.5) * 2
     check_attend(B, plain, q, cu, lens, make_table(rs, lens, page, pages), causal, kind)
+
+
+LONG = [  # requests of more rows than the narrow kernel takes, beside short ones; the last ones are divided over the tokens
+    ([300], [300], True), ([257, 3], [400, 90], True), ([1, 385, 0, 40], [77, 385, 50, 200], True), ([270], [100], False),
+    ([300, 300], [64, 0], False), ([260], [5000], True), ([400], [3], True), ([513, 2], [2500, 3100], False)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code,kind", [("int8", "fp32"), ("int8", "bf16"), ("e4m3", "fp16"), ("e4m3", "fp32")])
+@pytest.mark.parametrize("case", range(len(LONG)))
+@pytest.mark.parametrize("page,heads,group,dim", [(32, 2, 1, 32), (64, 1, 2, 64), (128, 1, 1, 128), (32, 1, 3, 128)])
+def test_attend_long_requests(B, code, kind, case, page, heads, group, dim):
+    n, lens, causal = LONG[case]
+    rs = np.random.RandomState(case * 5 + dim + page)
+    pages = sum(-(-x // page) for x in lens) + 3
+    plain = random_pool(rs, pages, heads, dim, page, code)
+    cu = np.concatenate([[0], np.cumsum(n)])
+    q = dense(rs, int(cu[-1]), heads * group, dim, kind, 0.5) * 2
+    check_attend(B, plain, q, cu, lens, make_table(rs, lens, page, pages), causal, kind)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_attend_long_requests_absent_pages_and_nan_codes(B, code):
+    """The wide kernel's masks: codes behind the last token are NaN (e4m3), pages of the table are missing, whole stages of them."""
+    rs = np.random.RandomState(31)
+    page, dim = 32, 64
+    plain = random_pool(rs, 30, 1, dim, page, code)
+    lens, n = [300, 81], [300, 280]
+    table = make_table(rs, lens, page, 30, cols=11)
+    cu = np.array([0, 300, 580])
+    q = dense(rs, 580, 1, dim, "bf16", 0.5)
+    pool = plain.to_device(B)
+    if code == "e4m3":
+        k, v = load_keys(pool.k.cpu().numpy()), load_values(pool.v.cpu().numpy())
+        for r, ln in enumerate(lens):
+            if ln % page:
+                k[table[r, ln // page], ln % page:], v[table[r, ln // page], ln % page:] = 0x7f, 0xff
+        pool.k.copy_(torch.from_numpy(store_keys(k)))
+        pool.v.copy_(torch.from_numpy(store_values(v)))
+    check_attend(B, plain, q, cu, lens, table, False, "bf16", pool=pool)
+    i = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=DEV)
+    t2 = table.copy()
+    for gone, bad in ((1, -1), (2, 30), (3, -2 ** 31), (4, 2 ** 31 - 1), (5, -1), (8, -7)):
+        t2[0, gone] = bad
+    left = [c for c in range(10) if t2[0, c] == table[0, c]]
+    kk = table.copy()
+    kk[0, :len(left)] = table[0, left]
+    want, wl, mean, most = attend64(plain, q.double().numpy(), cu, [32 * (len(left) - 1) + 300 % 32, 81], kk, False, 1 / math.sqrt(dim))
+    got = B.attend(pool, q.to(DEV), i(cu), i(lens), i(t2), causal=False)
+    tol, _ = attend_tolerance("bf16", dim, want, wl, mean, most)
+    assert (np.abs(got.cpu().double().numpy() - want) <= tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,lens", [([2, 1], [300, 900]), ([300, 4], [700, 1200])])
+def test_attend_rows_that_are_nan_or_infinite_stay_alone(B, n, lens):
+    """A query row with NaN or infinities is its own affair; the others get what they get without it."""
+    rs = np.random.RandomState(32)
+    plain = random_pool(rs, 50, 1, 64, 64, "int8")
+    cu = np.concatenate([[0], np.cumsum(n)])
+    table = make_table(rs, lens, 64, 50)
+    i = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=DEV)
+    for kind in TYPES:
+        q = dense(rs, int(cu[-1]), 2, 64, kind, 0.5).to(DEV)
+        pool = plain.to_device(B)
+        want = B.attend(pool, q, i(cu), i(lens), i(table), causal=False)
+        q[1, 0, 3], q[-1, 1, 7], q[0, 1, 0] = math.nan, math.inf, -math.inf
+        got = B.attend(pool, q, i(cu), i(lens), i(table), causal=False)
+        for r, h in ((1, 0), (cu[-1] - 1, 1), (0, 1)):
+            assert torch.isnan(got[r, h]).any()
+            got[r, h] = want[r, h]
+        assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_attend_overlapping_requests_stay_in_bounds(B):
+    """Row offsets that go back and forth are nobody's rows twice over: what is written is unspecified, where is not."""
+    rs = np.random.RandomState(33)
+    plain = random_pool(rs, 80, 1, 32, 32, "int8")
+    lens = [2000] * 7
+    table = np.tile(rs.permutation(80)[:63].astype(np.int32), (7, 1))
+    i = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=DEV)
+    for rows, hint in ((40, 1), (40, 40), (600, 600)):
+        q = dense(rs, rows, 2, 32, "fp16", 0.5).to(DEV)
+        big = torch.full((rows + 64, 2, 32), 5.0, dtype=torch.float16, device=DEV)
+        B.attend(plain.to_device(B), q, i([0, rows, 0, rows, 3, rows - 2, -8, 10 ** 9]), i(lens), i(table), max_q=hint, out=big[32:32 + rows])
+        assert torch.all(big[:32] == 5) and torch.all(big[32 + rows:] == 5)
+
+
+@pytest.mark.gpu
+def test_attend_captured_with_every_kernel_and_replayed(B):
+    """More than 64 requests, short and long ones: every launch of the read in one graph, replayed with other lengths in between."""
+    rs = np.random.RandomState(34)
+    reqs = 70
+    n = rs.randint(0, 3, reqs)
+    n[10], n[20] = 300, 40
+    lens = rs.randint(0, 200, reqs)
+    lens[10], lens[30] = 700, 1500
+    plain = random_pool(rs, 400, 1, 64, 64, "int8")
+    pool = plain.to_device(B)
+    cu = np.concatenate([[0], np.cumsum(n)])
+    i = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=DEV)
+    table, q, dlens, dcu = i(rs.randint(0, 400, (reqs, 24))), dense(rs, int(cu[-1]), 2, 64, "fp16", 0.5).to(DEV), i(lens), i(cu)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        B.attend(pool, q, dcu, dlens, table, with_lse=True)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o, z = B.attend(pool, q, dcu, dlens, table, with_lse=True)
+    for step in range(6):
+        dlens.copy_(i(rs.permutation(lens)))
+        q.copy_(dense(rs, int(cu[-1]), 2, 64, "fp16", 0.5))
+        g.replay()
+        torch.cuda.synchronize()
+        o2, z2 = B.attend(pool, q, dcu, dlens, table, with_lse=True)
+        assert torch.equal(o, o2) and torch.equal(z, z2)
+        torch.cuda.synchronize()
 
 
 @pytest.mark.gpu
