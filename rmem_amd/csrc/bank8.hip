@@ -223,7 +223,7 @@ __global__ __launch_bounds__(256) void mark_clear_kernel(rmem_bank8_append_args 
   const int row = blockIdx.x * 256 + threadIdx.x;
   if (row >= a.rows) return;
   const int slot = a.slots[row];
-  if (!in_pool(slot, a.bank)) return;
+  if (!in_pool(slot, a.bank) || goes_on(a.slots, row, slot, a.bank.page)) return;   // (each page that is reached has a run's begin)
   marks[slot >> ps].first = 0x7fffffff;
   marks[slot >> ps].runs = 0;
 }

@@ -882,7 +882,7 @@ __device__ __forceinline__ float over_groups(float x) {       // sum over the la
 }
 
 template <int ROWS, int D>
-__global__ __launch_bounds__(256) void attn_merge(rmem_bank8_attn_args a, Parts parts, Split sp) {
+__device__ __forceinline__ void merge(const rmem_bank8_attn_args& a, const Parts& parts, const Split& sp, int block, int blocks) {
   constexpr int WIDTH = D / 4, GROUPS = 64 / WIDTH, BLOCK = merge_block(ROWS), BLOCKS = ROWS / BLOCK;
   const int heads = a.bank.heads, lane = threadIdx.x & 63, G = sp.G;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -897,7 +897,7 @@ __global__ __launch_bounds__(256) void attn_merge(rmem_bank8_attn_args a, Parts 
       if (a.lse && d4 == 0) a.lse[at * a.heads_q + hq] = (__log2f(l) + m - LIFT) * LN2;
     }
   };
-  for (long item = blockIdx.x; item < items; item += gridDim.x) {
+  for (long item = block; item < items; item += blocks) {
     const long th = item / BLOCKS;
     const int h = (int)(th % heads), end = (int)(item % BLOCKS + 1) * BLOCK;
     const Split_tile t = parts.tiles[th / heads];
@@ -958,6 +958,17 @@ __global__ __launch_bounds__(256) void attn_merge(rmem_bank8_attn_args a, Parts 
   }
 }
 
+template <int ROWS, int D>
+__global__ __launch_bounds__(256) void attn_merge(rmem_bank8_attn_args a, Parts parts, Split sp) {
+  merge<ROWS, D>(a, parts, sp, blockIdx.x, gridDim.x);
+}
+// of the wide kernel's parts (the first `first` workgroups) and the narrow kernel's beside it: one launch instead of two, 4 us
+template <int D>
+__global__ __launch_bounds__(256) void attn_merge_both(rmem_bank8_attn_args a, Parts wide, Split wide_sp, Parts narrow, Split narrow_sp, int first) {
+  if ((int)blockIdx.x < first) merge<WROWS, D>(a, wide, wide_sp, blockIdx.x, first);
+  else merge<32, D>(a, narrow, narrow_sp, blockIdx.x - first, gridDim.x - first);
+}
+
 // -------------------------------------------------------------------------------------------------------------------- host
 constexpr int ROWS16 = 16;              // requests of at most this many rows per kv head take tiles of 16 rows
 // Up to this many the narrow kernel, beyond the wide one.  4 requests of 256 rows over 16 k tokens of 128 dims: narrow 61 us, wide 72;
@@ -969,9 +980,10 @@ constexpr int WIDE_CHUNK = 16;
 // Parts of all kv heads that a read is divided into.  Narrow: as many as workgroups fit the chip at once (registers), which a larger
 // number only adds starts and parts to merge to (64 ragged requests of 128 dims: 512 parts 100 us, 1024 101, 2048 104; of 32 dims 1536
 // parts 33, 512 39).  Wide: the same at 128 dims (512 rows over 64 k tokens: 512 parts 674 us, 2048 748); smaller dims have shorter
-// units, which even out what a causal mask makes uneven (4 x 2000 causal rows of 64 dims: 2048 parts 164, 512 185).
+// units, which even out what a causal mask makes uneven (4 x 2000 causal rows of 64 dims: 2048 parts 165, 1024 180, 512 187; 4 x 1674
+// rows of 32 dims over 1.7 to 8.4 k tokens: 1536 parts 135, 2048 144, 1024 144, 512 163).
 int narrow_units(int dim) { return dim == 128 ? 512 : dim == 64 ? 1024 : 1536; }
-int wide_units(int dim) { return dim == 128 ? 512 : 2048; }
+int wide_units(int dim) { return dim == 128 ? 512 : dim == 64 ? 2048 : 1536; }
 
 struct Launch {
   Split sp;
@@ -1038,24 +1050,25 @@ void launch_attn(const rmem_bank8_attn_args& a, const Parts& parts, const Launch
 }
 
 template <int D>
-int launch_dim(const rmem_bank8_attn_args& a, const Parts& parts, const Launch& l, hipStream_t s) {
+void launch_tiles(const rmem_bank8_attn_args& a, const Parts& parts, const Launch& l, hipStream_t s) {
   const bool e4m3 = a.bank.code == E4M3, two = a.type == FP32;
   if (e4m3) two ? launch_attn<D, E4M3, 2>(a, parts, l, s) : launch_attn<D, E4M3, 1>(a, parts, l, s);
   else two ? launch_attn<D, INT8, 2>(a, parts, l, s) : launch_attn<D, INT8, 1>(a, parts, l, s);
-  RMEM_CHECK_LAUNCH();
-  if (l.slots) {
-    const long tiles = l.tiles < l.sp.want ? l.tiles : l.sp.want;       // row tiles in at least two parts: at most `want`
-    const dim3 grid((unsigned)std::min(tiles * a.bank.heads * (l.rows / merge_block(l.rows)), 2048L));
-    if (l.rows == 16) hipLaunchKernelGGL((attn_merge<16, D>), grid, dim3(256), 0, s, a, parts, l.sp);
-    else if (l.rows == 32) hipLaunchKernelGGL((attn_merge<32, D>), grid, dim3(256), 0, s, a, parts, l.sp);
-    else hipLaunchKernelGGL((attn_merge<WROWS, D>), grid, dim3(256), 0, s, a, parts, l.sp);
-    RMEM_CHECK_LAUNCH();
-  }
-  return RMEM_OK;
 }
 
-int launch_read(const rmem_bank8_attn_args& a, float* ws, const Launch& l, hipStream_t s) {
-  Parts parts;
+int merge_grid(const rmem_bank8_attn_args& a, const Launch& l) {
+  const long tiles = l.tiles < l.sp.want ? l.tiles : l.sp.want;         // row tiles in at least two parts: at most `want`
+  return (int)std::min(tiles * a.bank.heads * (l.rows / merge_block(l.rows)), 2048L);
+}
+template <int D>
+void launch_merge(const rmem_bank8_attn_args& a, const Parts& parts, const Launch& l, hipStream_t s) {
+  const dim3 grid(merge_grid(a, l));
+  if (l.rows == 16) hipLaunchKernelGGL((attn_merge<16, D>), grid, dim3(256), 0, s, a, parts, l.sp);
+  else if (l.rows == 32) hipLaunchKernelGGL((attn_merge<32, D>), grid, dim3(256), 0, s, a, parts, l.sp);
+  else hipLaunchKernelGGL((attn_merge<WROWS, D>), grid, dim3(256), 0, s, a, parts, l.sp);
+}
+
+int place(const rmem_bank8_attn_args& a, float* ws, const Launch& l, Parts& parts, hipStream_t s) {
   parts.o = ws;
   parts.ml = ws + l.slots * a.bank.heads * l.rows * a.bank.dim;
   parts.tiles = reinterpret_cast<Split_tile*>(parts.ml + l.slots * a.bank.heads * l.rows * 2);
@@ -1070,7 +1083,33 @@ int launch_read(const rmem_bank8_attn_args& a, float* ws, const Launch& l, hipSt
     RMEM_CHECK_LAUNCH();
     parts.before = index;
   }
-  return a.bank.dim == 32 ? launch_dim<32>(a, parts, l, s) : a.bank.dim == 64 ? launch_dim<64>(a, parts, l, s) : launch_dim<128>(a, parts, l, s);
+  return RMEM_OK;
+}
+
+template <int D>
+int launch_dim(const rmem_bank8_attn_args& a, float* ws, const Plan& p, hipStream_t s) {
+  Parts wide, narrow;
+  if (p.wide.units) {
+    const int rc = place(a, ws, p.wide, wide, s);
+    if (rc != RMEM_OK) return rc;
+    launch_tiles<D>(a, wide, p.wide, s);
+    RMEM_CHECK_LAUNCH();
+    ws += part_floats(&a, p.wide);
+  }
+  if (p.narrow.units) {
+    const int rc = place(a, ws, p.narrow, narrow, s);
+    if (rc != RMEM_OK) return rc;
+    launch_tiles<D>(a, narrow, p.narrow, s);
+    RMEM_CHECK_LAUNCH();
+  }
+  const bool w = p.wide.units && p.wide.slots, n = p.narrow.units && p.narrow.slots;
+  if (w && n) {
+    const int first = merge_grid(a, p.wide);
+    hipLaunchKernelGGL((attn_merge_both<D>), dim3(first + merge_grid(a, p.narrow)), dim3(256), 0, s, a, wide, p.wide.sp, narrow, p.narrow.sp, first);
+  } else if (w) launch_merge<D>(a, wide, p.wide, s);
+  else if (n) launch_merge<D>(a, narrow, p.narrow, s);
+  RMEM_CHECK_LAUNCH();
+  return RMEM_OK;
 }
 
 }  // namespace
@@ -1091,10 +1130,5 @@ extern "C" int rmem_bank8_attn(const rmem_bank8_attn_args* a, void* stream) {
     return RMEM_ERR_INVALID;
   hipStream_t s = static_cast<hipStream_t>(stream);
   float* ws = static_cast<float*>(a->workspace);
-  if (p.wide.units) {
-    const int rc = launch_read(*a, ws, p.wide, s);
-    if (rc != RMEM_OK) return rc;
-    ws += part_floats(a, p.wide);
-  }
-  return p.narrow.units ? launch_read(*a, ws, p.narrow, s) : RMEM_OK;
+  return a->bank.dim == 32 ? launch_dim<32>(*a, ws, p, s) : a->bank.dim == 64 ? launch_dim<64>(*a, ws, p, s) : launch_dim<128>(*a, ws, p, s);
 }
