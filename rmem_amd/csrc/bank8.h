@@ -49,15 +49,24 @@ __device__ __forceinline__ float clean(float x, float top) {
   x = x == x ? x : 0.f;
   return __builtin_amdgcn_fmed3f(x, -top, top);
 }
-template <int CODE>
+// CLEAN false: the four are known to be finite and at most half a step beyond the largest code's value.
+template <int CODE, bool CLEAN = true>
 __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+#pragma clang fp contract(off)             // (a product that comes in is rounded before it is rounded to a code)
+  if constexpr (CLEAN) {
+    constexpr float top = CODE == INT8 ? 127.f : 448.f;
+    a = clean(a, top);
+    b = clean(b, top);
+    c = clean(c, top);
+    d = clean(d, top);
+  }
   if constexpr (CODE == INT8) {
-    const uint32_t x = __float_as_uint(clean(a, 127.f) + 12583040.f), y = __float_as_uint(clean(b, 127.f) + 12583040.f),
-                   z = __float_as_uint(clean(c, 127.f) + 12583040.f), w = __float_as_uint(clean(d, 127.f) + 12583040.f);
+    const uint32_t x = __float_as_uint(a + 12583040.f), y = __float_as_uint(b + 12583040.f),
+                   z = __float_as_uint(c + 12583040.f), w = __float_as_uint(d + 12583040.f);
     return __builtin_amdgcn_perm(__builtin_amdgcn_perm(w, z, 0x0c0c0400u), __builtin_amdgcn_perm(y, x, 0x0c0c0400u), 0x05040100u);
   } else {
-    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(clean(a, 448.f), clean(b, 448.f), 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(clean(c, 448.f), clean(d, 448.f), lo, true);
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
   }
 }
 // four code bytes -> their values
