@@ -469,6 +469,7 @@ int rmem_label_resize_nearest(const uint8_t *src, int32_t Hs, int32_t Ws, uint8_
  *
  * Element = code * scale.  code 0 ("int8"): integer -127..127, held as the byte code + 128; code 1 ("e4m3"): the bits of the
  * 8-bit float with 4 exponent and 3 mantissa bits, largest value 448, no infinities.  Scales are positive and finite.
+ * Codes of tokens that are held are numbers (append writes no NaN code); elsewhere in the pool NaN codes and scales do no harm.
  *   keys    [pages][heads][dim/16][page][16]
  *   values  [pages][heads][page/32][2][dim][16]   byte 4 m + r of half h = token 8 m + 4 h + r of the 32-token tile
  * slot = page_id * page + token in the page.  All pointers 16-byte aligned.  None of these calls is recordable (rmem_rec_*). */

@@ -228,7 +228,8 @@ def attend(pool: Pool, q: torch.Tensor, cu: torch.Tensor, lens: torch.Tensor, ta
         out = torch.empty((rows, heads_q, pool.dim), dtype=q.dtype, device=dev)
     else:
         _dense(out, "out", pool, heads_q, q)
-        _need((rows < 2 or out.stride(0) > 0) and (heads_q < 2 or out.stride(1) > 0), "out's rows and heads must not share memory")
+        (near, n), (far, m) = sorted(((out.stride(1), heads_q), (out.stride(0), rows)))
+        _need((n < 2 or near >= pool.dim) and (m < 2 or far >= (near * n if n > 1 else pool.dim)), "out's rows and heads must not share memory")
     if lse is not None:
         _need(isinstance(lse, torch.Tensor) and lse.dtype == torch.float32 and tuple(lse.shape) == (rows, heads_q) and lse.is_contiguous() and
               lse.device == dev, "lse must be a contiguous fp32 tensor [rows, query heads]")

@@ -118,7 +118,7 @@ __device__ __forceinline__ bool look_up(const rmem_bank8_attn_args& a, const Spl
   u.len = x.len;
   u.slot = b.slots + u.rt * u.ns;
   u.ord = b.ords + u.rt;
-  return u.rt >= 0;
+  return k >= 0 && u.rt >= 0;                  // (sums that row offsets which are none have wrapped)
 }
 
 template <int ROWS>
@@ -194,7 +194,7 @@ __device__ bool find_unit(const rmem_bank8_attn_args& a, const Split& sp, const 
   u.len = __builtin_amdgcn_readlane(x.len, l);
   u.slot = __builtin_amdgcn_readlane(s, l) - __builtin_amdgcn_readlane(split, l) + u.rt * u.ns;
   u.ord = __builtin_amdgcn_readlane(o, l) - __builtin_amdgcn_readlane(ord, l) + u.rt;
-  return true;
+  return k >= 0 && u.rt >= 0;
 }
 
 // row tiles in several parts
@@ -523,8 +523,8 @@ struct Parts {
 template <int ROWS, int R, int D>
 __device__ __forceinline__ void write_part(const Parts& w, const Acc<R, D>& c, const Unit& u, int h, int heads, int j, int g) {
   const int slot = u.slot + u.part;
-  if (slot >= w.slots) return;
-  if (h == 0 && u.part == 0 && j == 0 && g == 0 && u.ord < w.ords) {
+  if (slot < 0 || slot >= w.slots) return;
+  if (h == 0 && u.part == 0 && j == 0 && g == 0 && u.ord >= 0 && u.ord < w.ords) {
     const Split_tile t = {u.q0, u.n, u.rt, u.ns, u.slot, {0, 0, 0}};
     w.tiles[u.ord] = t;
   }
@@ -811,8 +811,8 @@ __global__ __launch_bounds__(256, NS == 2 && D == 128 ? 1 : 2) void attn_wide(rm
       } else {
         const int v = c - 4 * D, d = v % D, th = v / D;
         at = HALF + ((((th >> 1) * (D / 32) + (d >> 5)) * 4 + (th & 1)) << 5) + (d & 31);
-        if constexpr (CODE == E4M3) {            // NaN codes behind the last token
-          const int sub = __builtin_amdgcn_readfirstlane(th >> 1), left = u.len - (t0 + 2 * st + sub) * 32;
+        if constexpr (CODE == E4M3) {            // NaN codes behind the last token, or of the page read for an absent one
+          const int sub = __builtin_amdgcn_readfirstlane(th >> 1), left = (sub ? page1 : page0) < 0 ? 0 : u.len - (t0 + 2 * st + sub) * 32;
           if (left < 32) {
 #pragma unroll
             for (int m = 0; m < 4; ++m) x[m] = keep_first(x[m], left - 8 * m - 4 * (th & 1));

@@ -858,6 +858,48 @@ def test_attend_never_reads_what_is_not_there(B, causal):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("n,group", [(1, 1), (9, 2), (300, 1), (130, 4)])
+def test_attend_beside_pages_of_nan_codes(B, n, group, causal):
+    """Every page that no request names holds NaN codes and scales, the first one among them: absent pages, the last tile of a part and
+    the token behind the last one read nothing of them, in every kernel."""
+    rs = np.random.RandomState(n)
+    page, dim, pages = 32, 32, 40
+    plain = random_pool(rs, pages, 1, dim, page, "e4m3")
+    lens = [n + 289, n + 257]
+    held = [-(-x // page) for x in lens]
+    ids = 1 + rs.permutation(pages - 1)[:sum(held)]
+    table = np.full((2, max(held) + 2), -1, np.int64)
+    table[0, :held[0]], table[1, :held[1]] = ids[:held[0]], ids[held[0]:]
+    cu = np.array([0, n, 2 * n])
+    q = dense(rs, 2 * n, group, dim, "bf16", 0.5)
+    pool = plain.to_device(B)
+    k, v = load_keys(pool.k.cpu().numpy()), load_values(pool.v.cpu().numpy())
+    for r, ln in enumerate(lens):
+        if ln % page:
+            k[table[r, ln // page], ln % page:], v[table[r, ln // page], ln % page:] = 0x7f, 0xff
+    for pg in set(range(pages)) - set(ids.tolist()):
+        k[pg], v[pg] = 0x7f, 0x7f
+        pool.k_scale[pg] = math.nan
+        pool.v_scale[pg] = math.nan
+    pool.k.copy_(torch.from_numpy(store_keys(k)))
+    pool.v.copy_(torch.from_numpy(store_values(v)))
+    check_attend(B, plain, q, cu, lens, table, causal, "bf16", pool=pool)
+    i = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=DEV)
+    t2 = table.copy()
+    t2[0, 1], t2[1, 4] = -1, pages
+    if not causal:                                     # as if the tokens of the absent pages were left out
+        kk = np.full_like(table, -1)
+        kk[0, :held[0] - 1], kk[1, :held[1] - 1] = np.delete(table[0, :held[0]], 1), np.delete(table[1, :held[1]], 4)
+        want, wl, mean, most = attend64(plain, q.double().numpy(), cu, [x - page for x in lens], kk, False, 1 / math.sqrt(dim))
+        tol, _ = attend_tolerance("bf16", dim, want, wl, mean, most)
+        got = B.attend(pool, q.to(DEV), i(cu), i(lens), i(t2), causal=False)
+        assert (np.abs(got.cpu().double().numpy() - want) <= tol).all()
+    else:
+        assert torch.isfinite(B.attend(pool, q.to(DEV), i(cu), i(lens), i(t2), causal=True)).all()
+
+
+@pytest.mark.gpu
 def test_attend_lengths_beyond_the_table_and_odd_offsets(B):
     """Lengths are limited to the table's row, row offsets to the rows; rows that belong to nobody are left as they were."""
     rs = np.random.RandomState(13)
@@ -1065,3 +1107,24 @@ def test_two_streams_at_once(B):
     torch.cuda.synchronize()
     for w, g in zip(want, got):
         assert all(torch.equal(w, x) for x in g)
+
+
+@pytest.mark.gpu
+def test_attend_out_layouts(B):
+    """Rows and heads of `out` in either order, with gaps, of one row or head; refused where they overlap."""
+    f = lambda *s: torch.zeros(*s, dtype=torch.float16, device=DEV)
+    i = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    rs = np.random.RandomState(5)
+    plain = random_pool(rs, 4, 1, 64, 32, "int8")
+    pool, table = plain.to_device(B), i([[0, 1], [2, 3]])
+    q = dense(rs, 5, 3, 64, "fp16", 0.5).to(DEV)
+    args = (i([0, 2, 5]), i([40, 64]), table)
+    want = B.attend(pool, q, *args)
+    for out in (f(3, 5, 64).transpose(0, 1), f(5, 2, 3, 64)[:, 1], f(5, 3, 80)[:, :, 8:72], f(5, 200).as_strided((5, 3, 64), (200, 65, 1))):
+        assert B.attend(pool, q, *args, out=out) is out and torch.equal(out, want)
+    for out in (f(2000).as_strided((5, 3, 64), (64, 64, 1)), f(2000).as_strided((5, 3, 64), (191, 64, 1)), f(2000).as_strided((5, 3, 64), (192, 63, 1)),
+                f(2000).as_strided((5, 3, 64), (64, 319, 1))):
+        with pytest.raises(RmemError):
+            B.attend(pool, q, *args, out=out)
+    one = f(500).as_strided((1, 3, 64), (1, 64, 1))
+    assert torch.equal(B.attend(pool, q[:1], i([0, 1]), i([40]), table[:1], out=one), B.attend(pool, q[:1], i([0, 1]), i([40]), table[:1]))
