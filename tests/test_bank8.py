@@ -1112,6 +1112,7 @@ def test_two_streams_at_once(B):
 @pytest.mark.gpu
 def test_attend_out_layouts(B):
     """Rows and heads of `out` in either order, with gaps, of one row or head; refused where they overlap."""
+    from rmem_amd.hip import RmemError
     f = lambda *s: torch.zeros(*s, dtype=torch.float16, device=DEV)
     i = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
     rs = np.random.RandomState(5)
