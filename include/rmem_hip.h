@@ -538,6 +538,7 @@ int rmem_bank8_gather(const rmem_bank8_gather_args *a, void *stream);
  * elements and dim contiguous; lse [rows][heads_q] fp32 or NULL.  scale > 0.  max_rows: the largest number of rows of a request,
  * as far as known (it selects kernels; any value is safe).  Scores, weights and sums are fp32; q counts with 22 bits, values of
  * fp32 calls with 22-bit weights, of 16-bit calls with 11-bit weights.  Value scales below 2^-88 are read as 2^-88.
+ * (A request's value scales may differ by a factor of 2^100: beyond it the weights of the pages with the small ones would vanish.)
  * workspace: rmem_bank8_attn_workspace(a) bytes, 16-byte aligned, of this call alone until it has run. */
 typedef struct {
   rmem_bank8 bank;

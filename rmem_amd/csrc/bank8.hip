@@ -13,6 +13,7 @@ namespace {
 // One workgroup: the requests are scanned (pages asked for, rows, pages going back) up to 1024 at a time, the page ids that
 // move are spread over the threads by binary search in the scan.  Bound by the chain of dependent memory reads (lengths -> ring
 // and table entries), not by bytes; one workgroup keeps it one launch and lets state and lengths be updated in place.
+// 64 requests of one token 4.4 us; 500 with 17 k rows, 40 of them ending, 12 us and 4 us for the slot map.
 constexpr int PT = 1024;
 
 struct Scan3 {
@@ -283,19 +284,21 @@ __device__ __forceinline__ const T* element(const T* src, long ldr, int r, int a
 // them) leaves too few workgroups to hide the chain slots -> rows -> maximum -> codes.  Keys: a thread takes 16 dims of a token,
 // eight threads a token of 128 dims (256 bytes in, 128-byte pieces out).  Values: a thread takes 16 tokens (half a 32-token tile)
 // of two dims, so that a wave reads whole rows and each thread writes the two chunks that hold its tokens.
+// 25.6 k fp16 rows of 8 x 128 to e4m3: 48 us for 157 MB, 3.3 TB/s -- what is left is that chain, at 20 waves per CU (16: 50 us; 32 spill);
+// 64 single tokens 5.4 us.
 template <class T, int CODE, int D, bool FAST, int NT>
 __global__ __launch_bounds__(NT, 5) void append_kernel(rmem_bank8_append_args a, const PageMark* marks, int ps, int window) {
   __shared__ float s_max[NT / 64];
   __shared__ __attribute__((aligned(16))) int s_row[128];   // row that fills each place of the page, -1: none; the last of several
   __shared__ int s_other;
   const rmem_bank8& b = a.bank;
-  const int x = blockIdx.x, part = x >= b.heads, h = part ? x - b.heads : x;
+  const int zs = gridDim.z / 2, h = blockIdx.x, part = blockIdx.z >= zs;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int page = b.page;
   const T* src = static_cast<const T*>(part ? a.v : a.k) + (long)h * (part ? a.v_head : a.k_head);
   const long ldr = part ? a.v_row : a.k_row;
   // every wave looks the window's rows over at once: which of them begin a page that is this workgroup's to write
-  const int row0 = (blockIdx.z * GRID_Y + blockIdx.y) * window;
+  const int row0 = ((blockIdx.z - part * zs) * GRID_Y + blockIdx.y) * window;
   if (row0 >= a.rows) return;
   int w_slot = -1, w_runs = 0, w_ahead[2];             // slots of this lane's row and of those 64 and 128 behind it
   bool begins = false;
@@ -583,12 +586,13 @@ struct Append {
   static void run(const rmem_bank8_append_args& a, const PageMark* marks, int ps, int window, hipStream_t s) {
     // FAST: every row of every head begins on 16 bytes, and the rows span less than 4 GiB
     const unsigned long mis = (unsigned long)a.k | (unsigned long)a.v | (unsigned long)((a.k_row | a.k_head | a.v_row | a.v_head) * (long)sizeof(T));
-    // the heads of a window follow each other, so that what runs at a time reads whole rows (64 single tokens: 5.8 us, 6.6 head by head)
+    // a window's heads follow each other, so that what runs at a time reads whole rows; values after all keys (13 k rows of 8 x 32: 12.2 us,
+    // 12.7 head by head; 1000 single tokens of 8 x 128: 48 us, 55 with a window's keys and values side by side)
     const int windows = (a.rows + window - 1) / window;
-    const dim3 grid(2 * a.bank.heads, std::min(windows, GRID_Y), (windows + GRID_Y - 1) / GRID_Y);
+    const dim3 grid(a.bank.heads, std::min(windows, GRID_Y), 2 * ((windows + GRID_Y - 1) / GRID_Y));
     const long span = (a.rows - 1L) * std::max(a.k_row, a.v_row) + D;
     // Up to SCAN_ROWS rows most pages get a token or a few: workgroups of 128 keep more of their chains of reads in flight (1000
-    // single tokens: 47 us, 65 with 256); long calls fill whole pages, which 256 write faster (25 k tokens into pages of 128: 47, 56).
+    // single tokens: 48 us, 71 with 256); long calls fill whole pages, which 256 write faster (25 k tokens into pages of 128: 45, 52).
     if ((mis & 15) || span * (long)sizeof(T) >= 1L << 32) hipLaunchKernelGGL((append_kernel<T, CODE, D, false, 128>), grid, dim3(128), 0, s, a, marks, ps, window);
     else if (!marks) hipLaunchKernelGGL((append_kernel<T, CODE, D, true, 128>), grid, dim3(128), 0, s, a, marks, ps, window);
     else hipLaunchKernelGGL((append_kernel<T, CODE, D, true, 256>), grid, dim3(256), 0, s, a, marks, ps, window);
@@ -648,7 +652,7 @@ extern "C" int rmem_bank8_append(const rmem_bank8_append_args* a, void* stream) 
     RMEM_CHECK_LAUNCH();
   }
   // rows of a workgroup: one while that leaves the chip room (a step of single tokens), up to 64 of a long call's, most of whose
-  // rows begin no page (25 k rows of prompts: 63 us with up to 32, 52 us with up to 64)
+  // rows begin no page (25 k rows of prompts: 58 us with up to 32, 48 us with up to 64)
   const long groups = (long)a->rows * a->bank.heads * 2;
   const int window = groups <= APPEND_GROUPS ? 1 : groups >= 64L * APPEND_GROUPS ? 64 : (int)((groups + APPEND_GROUPS - 1) / APPEND_GROUPS);
   dispatch<Append>(a->type, a->bank.code, a->bank.dim, *a, marks, ps, window, s);

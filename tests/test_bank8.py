@@ -1129,3 +1129,27 @@ def test_attend_out_layouts(B):
             B.attend(pool, q, *args, out=out)
     one = f(500).as_strided((1, 3, 64), (1, 64, 1))
     assert torch.equal(B.attend(pool, q[:1], i([0, 1]), i([40]), table[:1], out=one), B.attend(pool, q[:1], i([0, 1]), i([40]), table[:1]))
+
+
+@pytest.mark.gpu
+def test_append_of_millions_of_rows(B):
+    """More windows than the grid's y holds: every row is written once and comes back within half a step of its page's scale."""
+    rows, page = 2_200_003, 128
+    pages = -(-rows // page) + 2
+    gen = torch.Generator(device=DEV).manual_seed(11)
+    x = torch.randn((rows, 2, 32), generator=gen, device=DEV, dtype=torch.float32).to(torch.bfloat16)
+    k, v = x[:, :1], x[:, 1:]
+    pool = B.Pool.empty(pages, 1, 32, page, "int8", DEV)
+    ids = torch.randperm(pages, generator=gen, device=DEV)
+    slots = (ids[:, None] * page + torch.arange(page, device=DEV)).reshape(-1)[:rows].to(torch.int32)
+    B.append(pool, k, v, slots)
+    got_k, got_v = B.gather(pool, slots, torch.float32)
+    for got, want, scale in ((got_k, k, pool.k_scale), (got_v, v, pool.v_scale)):
+        s = scale[(slots // page).long()][:, :, None]
+        pad = torch.zeros((pages * page - rows, 1, 32), device=DEV)
+        top = torch.cat([want.float().abs(), pad]).reshape(pages, -1).amax(1)[:-(-rows // page)]
+        at = ids[:-(-rows // page)]
+        # divided on the host: a device tensor over a number is a product with the number's inverse
+        assert np.array_equal(scale[at, 0].cpu().numpy(), top.cpu().numpy() / np.float32(127))
+        # half a step, and the roundings of 1 / s, the product and code * s: at most 127 codes times 3 * 2^-24, below 2^-15 of a step
+        assert ((got - want.float()).abs() <= s * (0.5 + 2.0 ** -14)).all()
