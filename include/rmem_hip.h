@@ -486,7 +486,9 @@ typedef struct {
  * A request that is not granted keeps lens = ctx and gets slots -1; it has to be asked for again.
  * had (or NULL): tokens each request held before; pages table[r][ceil(ctx/page)] .. table[r][ceil(had/page) - 1] go back to the
  * end of the ring, from where later calls take them (had > ctx: a request that ended or was cut).
- * free_ring [ring] with state = {head, count}: count free pages from position head on, modulo ring.  state_out may be state_in,
+ * free_ring [ring] with state = {head, count}: count free pages from position head on, modulo ring.  It has to have a place for
+ * every page that is in use (ring = the pool's pages always does): a page that goes back finds one among the ring - count that are
+ * not free at the call's begin, and is lost where there is none.  state_out may be state_in,
  * lens may be ctx.  rows >= the sum of add: slots past it are -1. */
 typedef struct {
   const int32_t *ctx, *add, *had; int32_t reqs;

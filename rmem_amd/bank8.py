@@ -114,7 +114,8 @@ def plan(ctx: torch.Tensor, add: torch.Tensor, table: torch.Tensor, free: torch.
     """Block tables, slot map and row offsets of one step (rmem_bank8_plan).
 
     ctx, add [reqs]: tokens that each request holds and wants added; table [reqs, pages per request]: its pages, extended in
-    place; free [ring] with state {position, count}: the free pages; rows: rows of the step (at least the sum of add, known to
+    place; free [ring] with state {position, count}: the free pages (as many places as the pool has pages: one that goes back and
+    finds none is lost); rows: rows of the step (at least the sum of add, known to
     the caller who packs them); had [reqs]: tokens held before, where requests ended or were cut -- their pages return to the
     ring in place.  A request whose pages are not to be had is left as it was (start -1, slots -1, counted in status[1]).
     `out` gives the results' tensors (a captured step: out.state may be `state`, out.lens may be `ctx`)."""

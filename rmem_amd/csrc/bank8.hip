@@ -116,7 +116,7 @@ __global__ __launch_bounds__(PT) void plan_kernel(rmem_bank8_plan_args p, int ps
       const int k = upper_bound(s_back, nr, i);
       const long long j = i - (k ? s_back[k - 1] : 0);
       const long long at = count + c_back + i;
-      if (at < p.ring)                                       // (more pages than the ring holds: returned twice, dropped)
+      if (at < p.ring)                                       // (more pages than the ring has places: dropped, and not counted)
         p.free_ring[ring_at(at)] = p.table[(base + k) * p.ld_table + s_held[k] + j];
     }
     if (n_back) __syncthreads();
@@ -170,9 +170,10 @@ __global__ __launch_bounds__(PT) void plan_kernel(rmem_bank8_plan_args p, int ps
       t += s_wave[0][w];
       m += s_wave[1][w];
     }
-    const long long left = count - t + c_back;
+    // what was written above: the places that this step's grants leave hold granted pages, which must not be counted as free
+    const long long held = count + c_back < p.ring ? count + c_back : p.ring;
     p.state_out[0] = (int)(head + t >= p.ring ? head + t - p.ring : head + t);
-    p.state_out[1] = (int)(left < p.ring ? left : p.ring);
+    p.state_out[1] = (int)(held - t);
     p.status[0] = (int)t;
     p.status[1] = (int)(m < 0x7fffffff ? m : 0x7fffffff);
   }

@@ -461,6 +461,51 @@ def test_plan_odd_values(B):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("places", ["none", "half", "one short", "all"])
+@pytest.mark.parametrize("reqs,page", [(2, 32), (40, 64), (300, 32), (1500, 32)])
+def test_plan_never_gives_a_page_to_two(B, reqs, page, places):
+    """Requests end, are cut and grow in one step, on rings with too few places for what goes back and with enough.  From lists,
+    without the ring's arithmetic: a page is held by one request or free once, grants take the free pages in order, and what goes back
+    stands behind the rest, as far as there were places that were not free."""
+    rs = np.random.RandomState(reqs + len(places))
+    up = lambda x: -(-x // page)
+    had = rs.randint(0, 9 * page, reqs)
+    had[0] = 5 * page
+    ctx = np.where(rs.rand(reqs) < 0.4, 0, np.where(rs.rand(reqs) < 0.3, had // 2, had))
+    ctx[0] = 0                                                   # one at least ends, one at least grows
+    add = np.where(rs.rand(reqs) < 0.5, rs.randint(0, 4 * page, reqs), 0)
+    add[-1] = 3 * page
+    had[-1] = ctx[-1] = min(had[-1], 4 * page)
+    cols = int(max(up(had).max(), up(ctx + add).max()))
+    held = up(had)
+    back_n, count = int(np.maximum(held - up(ctx), 0).sum()), int((up(ctx + add) - up(ctx)).sum()) + 2
+    ring = count + {"none": 0, "half": back_n // 2, "one short": back_n - 1, "all": back_n}[places]
+    ids = rs.permutation(int(held.sum()) + count)
+    table = np.full((reqs, cols), -1, np.int32)
+    at = count
+    for r in range(reqs):
+        table[r, :held[r]] = ids[at:at + held[r]]
+        at += held[r]
+    head = rs.randint(ring)
+    free = np.full(ring, -1, np.int32)
+    free[(head + np.arange(count)) % ring] = ids[:count]
+    was_free = ids[:count].tolist()
+    back = [int(table[r, c]) for r in range(reqs) for c in range(up(ctx[r]), held[r])]
+    d = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=DEV)
+    t, f = d(table), d(free)
+    p = B.plan(d(ctx), d(add), t, f, d([head, count]), page=page, rows=int(add.sum()), had=d(had))
+    t, f, lens, state = t.cpu().numpy(), f.cpu().numpy(), p.lens.cpu().numpy(), p.state.cpu().tolist()
+    assert np.array_equal(lens, ctx + add) and p.status.cpu().tolist() == [count - 2, 0]
+    new = [int(t[r, c]) for r in range(reqs) for c in range(up(ctx[r]), up(lens[r]))]
+    kept = [int(t[r, c]) for r in range(reqs) for c in range(up(ctx[r]))]
+    assert kept == [int(table[r, c]) for r in range(reqs) for c in range(up(ctx[r]))]
+    assert new == was_free[:count - 2]
+    now_free = f[(state[0] + np.arange(state[1])) % ring].tolist()
+    assert len(set(kept + new + now_free)) == len(kept + new + now_free)
+    assert now_free == was_free[count - 2:] + back[:ring - count]
+
+
+@pytest.mark.gpu
 def test_plan_in_place_step_by_step(B):
     """The state and the lengths updated in place over many steps; every page is held once at all times."""
     page, reqs, pages = 32, 5, 40
