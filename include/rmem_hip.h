@@ -535,7 +535,8 @@ int rmem_bank8_gather(const rmem_bank8_gather_args *a, void *stream);
 /* out_i = sum_j softmax_j(scale * q_i . k_j) v_j over the tokens j that row i sees; lse_i = log sum_j exp(scale * q_i . k_j).
  * Request r's rows are cu[r] .. cu[r+1] (limited to rows), its tokens the first lens[r] of its row of the table (limited to
  * cols * page).  causal: row i of n sees tokens j <= len - n + i, otherwise all.  A row that sees nothing gets 0 and -inf; rows
- * past cu[reqs] are left as they were.  A table entry outside the pool stands for a page that nobody sees.
+ * past cu[reqs] are left as they were.  A table entry outside the pool stands for a page that nobody sees.  (Rows of a request that
+ * rmem_bank8_plan did not grant are not in the bank, while its lens still counts what it had before: pass 0 for it.)
  * heads_q = a multiple of bank.heads: query head h reads head h / (heads_q / bank.heads).  q, out of `type` with strides in
  * elements and dim contiguous; lse [rows][heads_q] fp32 or NULL.  scale > 0.  max_rows: the largest number of rows of a request,
  * as far as known (it selects kernels; any value is safe).  Scores, weights and sums are fp32; q counts with 22 bits, values of

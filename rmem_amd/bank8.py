@@ -5,7 +5,7 @@ requests of any length share a pool; a step is
 
     p = plan(ctx, add, table, free, state, page=pool.page, rows=T)     # pages, slots and row offsets, on the device
     append(pool, k, v, p.slots)                                        # the new tokens, 8 bits
-    out, lse = attend(pool, q, p.cu, p.lens, table, with_lse=True)     # each request's rows over its pages
+    out, lse = attend(pool, q, p.cu, p.lens, table, start=p.start, with_lse=True)   # each request's rows over its pages
 
 and ``gather`` reads tokens back as dense rows.  Nothing is read back to the host and nothing synchronises, so a step can be
 captured in a hipGraph.  Calls run on torch's current stream of the pool's device, whichever device is current.  Arguments are
@@ -204,12 +204,14 @@ def gather(pool: Pool, slots: torch.Tensor, dtype: torch.dtype = torch.float32) 
 
 def attend(pool: Pool, q: torch.Tensor, cu: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, *, max_q: Optional[int] = None,
            causal: bool = True, scale: Optional[float] = None, out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
-           with_lse: bool = False, workspace: Optional[torch.Tensor] = None):
+           with_lse: bool = False, workspace: Optional[torch.Tensor] = None, start: Optional[torch.Tensor] = None):
     """Attention of each request's rows over its pages (rmem_bank8_attn).
 
     q [rows, query heads, dim] (query heads a multiple of the pool's; head h reads kv head h // group); cu [reqs + 1]: request
     r's rows; lens [reqs]: its tokens; table [reqs, pages per request]: their pages.  causal: a request's rows are its last
     tokens and see what is not behind them; otherwise every row sees every token.  A row that sees nothing gets 0 (and -inf).
+    start [reqs]: plan's -- the rows of a request that was not granted (start < 0) are not in the bank and see nothing; without it
+    they count as the last of the tokens that the request had before.
     scale defaults to 1 / sqrt(dim).  max_q: the largest number of rows of one request where known -- it selects kernels, any
     value is safe.  Rows behind the last request are not written: pass `out` (and `lse` [rows, query heads] fp32) where they
     matter.  workspace: uint8 scratch of this call alone, allocated where it is not given.
@@ -223,6 +225,9 @@ def attend(pool: Pool, q: torch.Tensor, cu: torch.Tensor, lens: torch.Tensor, ta
     _ints(lens, "lens", (reqs,), dev)
     _ints(cu, "cu", (reqs + 1,), dev)
     _table(table, reqs, pool.page, dev)
+    if start is not None:
+        _ints(start, "start", (reqs,), dev)
+        lens = lens.masked_fill(start < 0, 0)
     scale = 1.0 / math.sqrt(pool.dim) if scale is None else float(scale)
     _need(0.0 < scale < 3e38, "scale must be positive and finite")
     if out is None:

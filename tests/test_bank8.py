@@ -1129,6 +1129,78 @@ def test_a_captured_step_replayed(B, code, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("most", [4, 300])
+def test_rows_of_requests_that_were_not_granted_see_nothing(B, most, causal):
+    """A step on a short ring, eager and captured: with plan's `start` the rows of a request that found no page get 0 and -inf, all
+    others what the 64-bit attention gives; the same graph replayed once the ring has pages grants them."""
+    rs = np.random.RandomState(most)
+    page, heads, group, dim, pages, reqs = 32, 1, 2, 64, 60, 4
+    plain = random_pool(rs, pages, heads, dim, page, "int8")
+    ctx, add = np.array([64, 40, 64, 96]), np.array([2, most, 3, 1])
+    table = make_table(rs, ctx, page, 12, cols=20)
+    spare = [p for p in range(pages) if p not in table]
+    rows = int(add.sum())
+    i = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=DEV)
+    e = lambda n: torch.zeros(n, dtype=torch.int32, device=DEV)
+    pool, dt, dlens, state = plain.to_device(B), i(table), i(ctx), i([0, 0])
+    free = i(spare + [-1] * (pages - len(spare)))
+    k, v, q = (dense(rs, rows, h, dim, "fp16", 0.4) for h in (heads, heads, heads * group))
+    dk, dv, dq, dadd = k.to(DEV), v.to(DEV), q.to(DEV), i(add)
+
+    def step(out):
+        p = B.plan(dlens, dadd, dt, free, state, page=page, rows=rows, out=out)
+        B.append(pool, dk, dv, p.slots)
+        return p, *B.attend(pool, dq, p.cu, p.lens, dt, start=p.start, causal=causal, max_q=most, with_lse=True)
+
+    mine = B.Plan(e(reqs + 1), e(reqs), e(reqs), e(rows), e(2), e(2))
+    start = [t.clone() for t in (pool.k, pool.v, pool.k_scale, pool.v_scale)]
+
+    def check(p, o, lse, few):
+        st, ln, cu = p.start.cpu().numpy(), p.lens.cpu().numpy(), p.cu.cpu().numpy()
+        # four tokens fit into request 1's page; the others ask for one page, and of two free ones 0 takes the first
+        want_on = (np.array([True, most == 4, most == 4, False]) if few else np.ones(4, bool))
+        assert np.array_equal(st >= 0, want_on)
+        now = PlainPool(pages, heads, dim, page, "int8")
+        for w in "kv":
+            now.codes[w], now.scale[w] = plain.codes[w].copy(), plain.scale[w].copy()
+        now.append(to_np(k), to_np(v), p.slots.cpu().numpy())
+        want, wl, mean, tops = attend64(now, q.double().numpy(), cu, np.where(want_on, ln, 0), dt.cpu().numpy(), causal, 1 / math.sqrt(dim))
+        tol, tol_lse = attend_tolerance("fp16", dim, want, wl, mean, tops)
+        o, lse = o.cpu().double().numpy(), lse.cpu().double().numpy()
+        assert (np.abs(o - want) <= tol).all()
+        for r in range(reqs):
+            part = slice(cu[r], cu[r + 1])
+            assert want_on[r] or ((o[part] == 0).all() and (lse[part] == -np.inf).all())
+            assert not want_on[r] or (np.abs(lse[part] - wl[part]) <= tol_lse[part]).all()
+
+    def reset(count):
+        for t, x in zip((pool.k, pool.v, pool.k_scale, pool.v_scale), start):
+            t.copy_(x)
+        dt.copy_(i(table))
+        state.copy_(i([0, count]))
+
+    for bad in (mine.start[:2], mine.start.long(), mine.start.cpu(), [0] * reqs):
+        with pytest.raises(B.RmemError):
+            B.attend(pool, dq, mine.cu, mine.lens, dt, start=bad)
+    reset(2)
+    check(*step(mine), True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(mine)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step(mine)
+    for count in (2, len(spare), 2, len(spare)):
+        reset(count)
+        g.replay()
+        torch.cuda.synchronize()
+        check(*got, count == 2)
+
+
+@pytest.mark.gpu
 def test_two_streams_at_once(B):
     """Two pools on two streams, calls interleaved on the host: no buffer is shared behind the caller's back."""
     rs = np.random.RandomState(23)
