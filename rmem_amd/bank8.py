@@ -11,6 +11,7 @@ and ``gather`` reads tokens back as dense rows.  Nothing is read back to the hos
 captured in a hipGraph.  Calls run on torch's current stream of the pool's device, whichever device is current.  Arguments are
 checked on the host (`RmemError`); lengths, slots and page ids live on the device, where values outside the pool are skipped.
 The caller orders calls on one pool (one stream, or events between streams), as for any tensor that is updated in place.
+There is no backward pass: tensors that require grad are refused where gradients are recorded.
 """
 from __future__ import annotations
 
@@ -153,6 +154,8 @@ def _dense(t, name: str, pool: Pool, heads: int, like: Optional[torch.Tensor] = 
         _refuse(f"{name}'s last dimension must be contiguous")
     if like is not None and (t.dtype != like.dtype or t.shape != like.shape):
         _refuse(f"{name} must have its partner's type and shape")
+    if t.requires_grad and torch.is_grad_enabled():
+        _refuse(f"{name} requires grad, and codes have none: call under torch.no_grad() or with a detached tensor")
 
 
 def _workspace(given: Optional[torch.Tensor], need: int, device) -> Optional[torch.Tensor]:

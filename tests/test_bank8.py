@@ -323,6 +323,42 @@ def test_python_refuses_host_tensors_and_bad_choices():
         bank8.attend(None, z(1), i(2), i(1), i(1, 1))
 
 
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda:0", marks=pytest.mark.gpu)])
+def test_tensors_that_require_grad_are_refused(dev):
+    """Codes carry no gradient, so a graph would be cut without a word; under no_grad, or detached, the same tensors are taken."""
+    from types import SimpleNamespace
+    from rmem_amd import bank8
+    from rmem_amd.hip import RmemError
+    f = lambda *s, grad=False: torch.ones(*s, dtype=torch.float16, device=dev, requires_grad=grad)
+    plain, leaf = f(3, 2, 64), f(3, 2, 64, grad=True)
+    if dev == "cpu":                                   # the check itself: pools live on a device
+        pool = SimpleNamespace(device=plain.device, dim=64)
+        for t in (leaf, leaf * 2):
+            with pytest.raises(RmemError, match="grad"):
+                bank8._dense(t, "k", pool, 2)
+            with torch.no_grad():
+                bank8._dense(t, "k", pool, 2)
+            bank8._dense(t.detach(), "k", pool, 2)
+        bank8._dense(plain, "k", pool, 2)
+        return
+    i = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)
+    pool = bank8.Pool.empty(2, 2, 64, 32, "int8", dev)
+    slots, args = i(0, 1, 2), (i(0, 3), i(3), torch.zeros(1, 2, dtype=torch.int32, device=dev))
+    before = pool.k.clone()
+    for bad in ((leaf, plain), (plain, leaf)):
+        with pytest.raises(RmemError, match="grad"):
+            bank8.append(pool, *bad, slots)
+    assert torch.equal(pool.k, before)
+    with torch.no_grad():
+        bank8.append(pool, leaf, leaf, slots)
+        want = bank8.attend(pool, leaf, *args)
+    for kw in (dict(q=leaf), dict(q=plain, out=leaf)):
+        with pytest.raises(RmemError, match="grad"):
+            bank8.attend(pool, kw["q"], *args, out=kw.get("out"))
+    got = bank8.attend(pool, leaf.detach(), *args)
+    assert torch.equal(got, want) and not got.requires_grad
+
+
 @pytest.mark.gpu
 def test_python_refuses_mismatched_device_tensors(B):
     from rmem_amd.hip import RmemError
