@@ -158,6 +158,14 @@ def _dense(t, name: str, pool: Pool, heads: int, like: Optional[torch.Tensor] = 
         _refuse(f"{name} requires grad, and codes have none: call under torch.no_grad() or with a detached tensor")
 
 
+def _apart(t: torch.Tensor) -> bool:
+    """Whether no two elements of t [rows, heads, dim] lie in one place: the dimension of the smaller step spans that many steps but
+    one and a vector, and the other one steps over at least this."""
+    (near, n), (far, m) = sorted(((t.stride(1), t.shape[1]), (t.stride(0), t.shape[0])))
+    block = near * (n - 1) + t.shape[2]
+    return (n < 2 or near >= t.shape[2]) and (m < 2 or far >= block)
+
+
 def _workspace(given: Optional[torch.Tensor], need: int, device) -> Optional[torch.Tensor]:
     """Scratch of one call: the caller's, or a new tensor (stream-ordered allocator, or the graph's pool while capturing)."""
     _need(need >= 0, "arguments refused")
@@ -237,8 +245,7 @@ def attend(pool: Pool, q: torch.Tensor, cu: torch.Tensor, lens: torch.Tensor, ta
         out = torch.empty((rows, heads_q, pool.dim), dtype=q.dtype, device=dev)
     else:
         _dense(out, "out", pool, heads_q, q)
-        (near, n), (far, m) = sorted(((out.stride(1), heads_q), (out.stride(0), rows)))
-        _need((n < 2 or near >= pool.dim) and (m < 2 or far >= (near * n if n > 1 else pool.dim)), "out's rows and heads must not share memory")
+        _need(_apart(out), "out's rows and heads must lie apart: the larger step at least the extent of the other dimension")
     if lse is not None:
         _need(isinstance(lse, torch.Tensor) and lse.dtype == torch.float32 and tuple(lse.shape) == (rows, heads_q) and lse.is_contiguous() and
               lse.device == dev, "lse must be a contiguous fp32 tensor [rows, query heads]")

@@ -359,6 +359,24 @@ def test_tensors_that_require_grad_are_refused(dev):
     assert torch.equal(got, want) and not got.requires_grad
 
 
+def test_out_layouts_that_lie_apart():
+    """Every step and size of a small range: what is taken shares no memory, and what nests is taken -- also rows that begin right
+    behind the last head's end, with gaps between heads."""
+    from rmem_amd import bank8
+    buf, dim = torch.zeros(200), 3
+    for rows in range(1, 5):
+        for heads in range(1, 5):
+            for row in range(0, 24):
+                for head in range(0, 24):
+                    t = buf.as_strided((rows, heads, dim), (row, head, 1))
+                    at = (torch.arange(rows)[:, None, None] * row + torch.arange(heads)[None, :, None] * head + torch.arange(dim)).flatten()
+                    apart, nested = at.unique().numel() == at.numel(), False
+                    for (a, n), (b, m) in (((row, rows), (head, heads)), ((head, heads), (row, rows))):
+                        nested |= (n == 1 or a >= dim) and (m == 1 or b >= a * (n - 1) + dim)
+                    assert not nested or apart
+                    assert bank8._apart(t) == nested, (rows, heads, row, head)
+
+
 @pytest.mark.gpu
 def test_python_refuses_mismatched_device_tensors(B):
     from rmem_amd.hip import RmemError
@@ -1282,6 +1300,24 @@ def test_attend_out_layouts(B):
             B.attend(pool, q, *args, out=out)
     one = f(500).as_strided((1, 3, 64), (1, 64, 1))
     assert torch.equal(B.attend(pool, q[:1], i([0, 1]), i([40]), table[:1], out=one), B.attend(pool, q[:1], i([0, 1]), i([40]), table[:1]))
+
+
+@pytest.mark.gpu
+def test_attend_out_rows_right_behind_the_last_head(B):
+    """Heads with gaps between them, rows without (the next row begins where the last head ends): shares no memory, so it is taken."""
+    f = lambda *s: torch.zeros(*s, dtype=torch.float16, device=DEV)
+    i = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    rs = np.random.RandomState(6)
+    pool = random_pool(rs, 4, 1, 64, 32, "int8").to_device(B)
+    q = dense(rs, 5, 3, 64, "fp16", 0.5).to(DEV)
+    args = (i([0, 2, 5]), i([40, 64]), i([[0, 1], [2, 3]]))
+    want = B.attend(pool, q, *args)
+    for row, head in ((224, 80), (80, 5 * 80 - 16), (193, 64)):
+        buf = f(2000).fill_(9)
+        out = buf.as_strided((5, 3, 64), (row, head, 1))
+        assert B.attend(pool, q, *args, out=out) is out and torch.equal(out, want)
+        out.fill_(9)
+        assert torch.all(buf == 9)                      # nothing beside it
 
 
 @pytest.mark.gpu
