@@ -517,14 +517,14 @@ typedef struct {
   rmem_bank8 bank;
   const void *k, *v; int32_t type;
   int64_t k_row, k_head, v_row, v_head;             /* strides of row and head */
-  const int32_t *slots; int32_t rows;               /* rows < 2^24 */
+  const int32_t *slots; int32_t rows;               /* rows < 2^24, bank.heads < 2^16 */
   void *workspace; int64_t workspace_bytes;
 } rmem_bank8_append_args;
 int64_t rmem_bank8_append_workspace(const rmem_bank8_append_args *a);   /* -1: invalid arguments */
 int rmem_bank8_append(const rmem_bank8_append_args *a, void *stream);
 
 /* out[row] = code * scale of slot slots[row], rounded to `type`; zeros where the slot lies outside the pool.
- * ko, vo: [rows][heads][dim], contiguous, 16-byte aligned. */
+ * ko, vo: [rows][heads][dim], contiguous, 16-byte aligned.  rows < 2^30, bank.heads < 2^16. */
 typedef struct {
   rmem_bank8 bank;
   const int32_t *slots; int32_t rows;
@@ -542,6 +542,9 @@ int rmem_bank8_gather(const rmem_bank8_gather_args *a, void *stream);
  * as far as known (it selects kernels; any value is safe).  Scores, weights and sums are fp32; q counts with 22 bits, values of
  * fp32 calls with 22-bit weights, of 16-bit calls with 11-bit weights.  Value scales below 2^-88 are read as 2^-88.
  * (A request's value scales may differ by a factor of 2^100: beyond it the weights of the pages with the small ones would vanish.)
+ * Refused: launches of 2^24 workgroups or more.  With G = heads_q / bank.heads a launch has, for each of bank.heads, rows * G / T of
+ * them, min(reqs, rows) for tiles that are not full, and up to 2048 in all (at least one for each head) for what is divided; T = 16
+ * with max_rows * G up to 16, 32 up to 256, beyond it two launches, T = 128 and, of several requests, T = 32.
  * workspace: rmem_bank8_attn_workspace(a) bytes, 16-byte aligned, of this call alone until it has run. */
 typedef struct {
   rmem_bank8 bank;

@@ -168,7 +168,7 @@ def _apart(t: torch.Tensor) -> bool:
 
 def _workspace(given: Optional[torch.Tensor], need: int, device) -> Optional[torch.Tensor]:
     """Scratch of one call: the caller's, or a new tensor (stream-ordered allocator, or the graph's pool while capturing)."""
-    _need(need >= 0, "arguments refused")
+    _need(need >= 0, "sizes refused (limits of one call: include/rmem_hip.h)")
     if given is None:
         return torch.empty(need, dtype=torch.uint8, device=device) if need else None
     if not (isinstance(given, torch.Tensor) and given.dtype == torch.uint8 and given.is_contiguous() and given.device == device and
@@ -226,6 +226,7 @@ def attend(pool: Pool, q: torch.Tensor, cu: torch.Tensor, lens: torch.Tensor, ta
     scale defaults to 1 / sqrt(dim).  max_q: the largest number of rows of one request where known -- it selects kernels, any
     value is safe.  Rows behind the last request are not written: pass `out` (and `lse` [rows, query heads] fp32) where they
     matter.  workspace: uint8 scratch of this call alone, allocated where it is not given.
+    A call that would need 2^24 workgroups (1.4 million single rows of 64 query heads over 8, for instance) is refused: divide it.
     Returns out, or (out, lse) with `with_lse` or `lse`."""
     _need(isinstance(pool, Pool), "pool must be a Pool")
     if not (isinstance(q, torch.Tensor) and q.dim() == 3 and q.shape[1] > 0 and q.shape[1] % pool.heads == 0):

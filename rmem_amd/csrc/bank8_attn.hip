@@ -1038,6 +1038,12 @@ Plan make_plan(const rmem_bank8_attn_args* a) {
   return p;
 }
 
+// A launch of 256 threads per workgroup counts its threads in 32 bits.
+constexpr long MOST_GROUPS = 1L << 24;
+bool fits_grids(const rmem_bank8_attn_args* a, const Plan& p) {
+  return p.narrow.units * a->bank.heads < MOST_GROUPS && p.wide.units * a->bank.heads < MOST_GROUPS;
+}
+
 // floats of a launch's workspace: partial results, references and sums, tiles in several parts (at most `want`: two parts each),
 // the division's index; each a multiple of 16 bytes
 long part_floats(const rmem_bank8_attn_args* a, const Launch& l) {
@@ -1121,6 +1127,7 @@ int launch_dim(const rmem_bank8_attn_args& a, float* ws, const Plan& p, hipStrea
 extern "C" int64_t rmem_bank8_attn_workspace(const rmem_bank8_attn_args* a) {
   if (!valid_attn(a)) return -1;
   const Plan p = make_plan(a);
+  if (!fits_grids(a, p)) return -1;
   return 4 * ((p.narrow.units ? part_floats(a, p.narrow) : 0) + (p.wide.units ? part_floats(a, p.wide) : 0));
 }
 
@@ -1129,8 +1136,8 @@ extern "C" int rmem_bank8_attn(const rmem_bank8_attn_args* a, void* stream) {
   if (a->rows == 0) return RMEM_OK;
   const Plan p = make_plan(a);
   const int64_t need = rmem_bank8_attn_workspace(a);
-  if (!a->q || !a->out || !a->cu || !a->lens || !a->table ||
-      (need && (!a->workspace || ((uintptr_t)a->workspace % 16) || a->workspace_bytes < need)) || p.narrow.units * a->bank.heads >= 1 << 24 || p.wide.units * a->bank.heads >= 1 << 24)
+  if (need < 0 || !a->q || !a->out || !a->cu || !a->lens || !a->table ||
+      (need && (!a->workspace || ((uintptr_t)a->workspace % 16) || a->workspace_bytes < need)))
     return RMEM_ERR_INVALID;
   hipStream_t s = static_cast<hipStream_t>(stream);
   float* ws = static_cast<float*>(a->workspace);

@@ -304,6 +304,26 @@ def test_c_abi_refuses_bad_arguments():
         assert lib.rmem_bank8_attn(C.byref(a), None) == -1, bad
 
 
+@pytest.mark.parametrize("heads,group,longest,each", [(8, 1, 1, 1 + 1 / 16), (8, 8, 1, 1 + 8 / 16), (64, 1, 100, 1 + 1 / 32), (1, 1, 300, 1 + 1 / 32),
+                                                      (128, 4, 1, 1 + 4 / 16)])
+def test_c_abi_refuses_reads_of_too_many_workgroups(heads, group, longest, each):
+    """A request of its own for every row: heads * (rows * each + parts) workgroups, which have to stay below 2^24.  The workspace's
+    size and the call agree; the limit is where the header puts it, up to the parts of what is divided.  (With longest * group above
+    256 a call makes a launch of tiles of 128 rows and one of 32, of which the latter has more workgroups.)"""
+    from rmem_amd import hip
+    lib = hip.load()
+
+    def args(rows):
+        return hip.Bank8AttnArgs(_bank(hip, heads=heads), _addr(4), _addr(5), None, 1, heads * group * 64, 64, heads * group * 64, 64, _addr(6), _addr(7),
+                                 rows, rows, _addr(8), 4, 4, heads * group, longest, 1, 0.1, _addr(20), 1 << 60)
+
+    limit = 2 ** 24 / heads / each
+    parts = max(2048, heads) / heads
+    fits, not_fits = args(int(limit - parts - 2)), args(int(limit + 2))
+    assert lib.rmem_bank8_attn_workspace(C.byref(fits)) >= 0
+    assert lib.rmem_bank8_attn_workspace(C.byref(not_fits)) == -1 and lib.rmem_bank8_attn(C.byref(not_fits), None) == -1
+
+
 def test_python_refuses_host_tensors_and_bad_choices():
     from rmem_amd import bank8, hip
     z = lambda *s, dt=torch.uint8: torch.zeros(*s, dtype=dt)
