@@ -25,28 +25,42 @@ EXTRA_FLAGS = {"mha.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
+def _commands() -> list:
+    """Every compile command and the link, in order."""
+    hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+    objs = [os.path.join(CSRC, src.replace(".hip", ".o")) for src in SOURCES]
+    cmds = [[hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-c", os.path.join(CSRC, src), "-o", obj] +
+            NO_PACKED_FP32 + EXTRA_FLAGS.get(src, []) + os.environ.get("RMEM_HIPCC_FLAGS", "").split() for src, obj in zip(SOURCES, objs)]
+    return cmds + [[hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs]
+
+
+def _stamp() -> str:
+    """The commands as the library keeps them beside itself (flags decide about its results as sources do), without where they ran."""
+    return "\n".join(" ".join(c) for c in _commands()).replace(CSRC + os.sep, "")
+
+
 def _stale() -> bool:
     if not os.path.exists(LIB):
         return True
     t = os.path.getmtime(LIB)
-    return any(os.path.getmtime(os.path.join(CSRC, f)) > t for f in SOURCES + HEADERS)
+    if any(os.path.getmtime(os.path.join(CSRC, f)) > t for f in SOURCES + HEADERS):
+        return True
+    try:
+        with open(LIB + ".cmd") as f:
+            return f.read() != _stamp()
+    except OSError:
+        return True
 
 
 def build_lib(force: bool = False, verbose: bool = False) -> str:
     if not force and not _stale():
         return LIB
-    hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    objs = []
-    for src in SOURCES:
-        obj = os.path.join(CSRC, src.replace(".hip", ".o"))
-        cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-c",
-               os.path.join(CSRC, src), "-o", obj] + NO_PACKED_FP32 + EXTRA_FLAGS.get(src, []) + os.environ.get("RMEM_HIPCC_FLAGS", "").split()
+    for cmd in _commands():
         if verbose:
             print(" ".join(cmd), file=sys.stderr)
         subprocess.check_call(cmd)
-        objs.append(obj)
-    cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs
-    subprocess.check_call(cmd)
+    with open(LIB + ".cmd", "w") as f:
+        f.write(_stamp())
     return LIB
 
 

@@ -686,3 +686,43 @@ def test_no_undefined_names_in_bench_and_package():
         sorted(glob.glob(os.path.join(root, "rmem_amd", "*.py"))) + sorted(glob.glob(os.path.join(root, "rmem_amd", "nets", "*.py")))
     bad = {os.path.relpath(f, root): _undefined_names(f) for f in files}
     assert not any(bad.values()), {k: v for k, v in bad.items() if v}
+
+
+def test_library_is_rebuilt_when_its_flags_change(tmp_path, monkeypatch):
+    """Up to date means: newer than every source and built by the same commands -- flags decide about results as sources do."""
+    from rmem_amd import build
+    csrc = tmp_path / "a" / "csrc"
+    csrc.mkdir(parents=True)
+    (tmp_path / "include").mkdir()
+    for f in build.SOURCES + build.HEADERS:
+        (csrc / f).write_text("")
+    log = tmp_path / "log"
+    compiler = tmp_path / "hipcc"                # notes that it was called and writes what -o names
+    compiler.write_text(f'#!/bin/sh\necho "$@" >> {log}\nwhile [ "$1" != -o ]; do shift; done\n: > "$2"\n')
+    compiler.chmod(0o755)
+    monkeypatch.setenv("HIPCC", str(compiler))
+    monkeypatch.delenv("RMEM_HIPCC_FLAGS", raising=False)
+    monkeypatch.setattr(build, "CSRC", str(csrc))
+    monkeypatch.setattr(build, "LIB", str(csrc / "librmem_hip.so"))
+
+    def runs():
+        if log.exists():
+            log.unlink()
+        build.build_lib()
+        return len(log.read_text().splitlines()) if log.exists() else 0
+
+    every = len(build.SOURCES) + 1
+    assert runs() == every and runs() == 0
+    monkeypatch.setenv("RMEM_HIPCC_FLAGS", "-DOTHER=1")
+    assert runs() == every and runs() == 0
+    monkeypatch.delenv("RMEM_HIPCC_FLAGS")
+    monkeypatch.setattr(build, "EXTRA_FLAGS", {})
+    assert runs() == every and runs() == 0
+    monkeypatch.setattr(build, "NO_PACKED_FP32", [])
+    assert runs() == every and runs() == 0
+    later = os.path.getmtime(build.LIB) + 10
+    os.utime(csrc / "bank8.h", (later, later))
+    assert runs() == every
+    os.utime(csrc / "bank8.h", (later - 100, later - 100))
+    os.remove(build.LIB + ".cmd")                # of unknown flags
+    assert runs() == every and runs() == 0
