@@ -1089,6 +1089,45 @@ def test_attend_results_do_not_depend_on_hints_or_neighbours(B):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["fp16", "fp32"])
+def test_attend_each_request_alone(B, kind):
+    """A batch whose requests go to the narrow and the wide kernel, and each of its requests in a call of its own: the division differs,
+    both are within tolerance of the 64-bit result."""
+    rs = np.random.RandomState(17)
+    plain = random_pool(rs, 60, 2, 64, 64, "e4m3")
+    lens, n = [1100, 40, 600, 450, 7], [40, 1, 2, 300, 0]
+    cu = np.concatenate([[0], np.cumsum(n)])
+    table = make_table(rs, lens, 64, 60)
+    q = dense(rs, int(cu[-1]), 4, 64, kind, 0.5)
+    pool = plain.to_device(B)
+    check_attend(B, plain, q, cu, lens, table, True, kind, pool=pool)
+    for r, rows in enumerate(n):
+        if rows:
+            check_attend(B, plain, q[cu[r]:cu[r + 1]], [0, rows], lens[r:r + 1], table[r:r + 1], True, kind, pool=pool)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,hint", [(40, 1), (40, 40), (600, 600)])
+def test_attend_many_overlapping_requests_stay_in_bounds(B, rows, hint):
+    """More than 64 requests (the division is looked up) whose row offsets go back and forth: what is written is unspecified, where is
+    not."""
+    rs = np.random.RandomState(rows + hint)
+    reqs = 70
+    pool = random_pool(rs, 80, 1, 32, 32, "int8").to_device(B)
+    i = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=DEV)
+    table = i(np.tile(rs.permutation(80)[:63], (reqs, 1)))
+    cu = rs.randint(-20, rows + 20, reqs + 1)
+    cu[::2] = 0
+    cu[5], cu[-1] = 10 ** 9, rows
+    q = dense(rs, rows, 2, 32, "fp16", 0.5).to(DEV)
+    big = torch.full((rows + 64, 2, 32), 5.0, dtype=torch.float16, device=DEV)
+    sums = torch.full((rows + 64, 2), 5.0, device=DEV)
+    B.attend(pool, q, i(cu), i(rs.randint(0, 2017, reqs)), table, max_q=hint, causal=False, out=big[32:32 + rows], lse=sums[32:32 + rows])
+    for t in (big, sums):
+        assert torch.all(t[:32] == 5) and torch.all(t[32 + rows:] == 5)
+
+
+@pytest.mark.gpu
 def test_offsets_beyond_32_bits(B):
     """A pool of more than 4 GiB of codes: pages at its end written, read back and attended to."""
     heads, dim, page = 8, 128, 128
@@ -1298,6 +1337,42 @@ def test_two_streams_at_once(B):
     torch.cuda.synchronize()
     for w, g in zip(want, got):
         assert all(torch.equal(w, x) for x in g)
+
+
+@pytest.mark.gpu
+def test_two_streams_of_long_calls_at_once(B):
+    """The calls that need scratch -- an append of more than 4096 rows in any order, a read of more than 64 requests, short and long
+    and divided over their tokens -- and a gather, on two streams at once: every result as on one stream, bit for bit."""
+    rs = np.random.RandomState(24)
+    i = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=DEV)
+    page, pages, heads, dim, reqs = 32, 160, 2, 64, 70
+
+    def job():
+        n, lens = rs.randint(0, 3, reqs), rs.randint(0, 200, reqs)
+        n[10], n[20], lens[10], lens[30] = 300, 40, 700, 1500
+        cu = np.concatenate([[0], np.cumsum(n)])
+        k, v = (dense(rs, pages * page, heads, dim, "bf16", 0.5).to(DEV) for _ in range(2))
+        q = dense(rs, int(cu[-1]), 2 * heads, dim, "bf16", 0.5).to(DEV)
+        return B.Pool.empty(pages, heads, dim, page, "int8", DEV), k, v, i(rs.permutation(pages * page)), q, i(cu), i(lens), i(rs.randint(0, pages, (reqs, 48)))
+
+    def work(pool, k, v, slots, q, cu, lens, table):
+        B.append(pool, k, v, slots)                    # (every page whole: it begins anew, the same each time)
+        return [*B.attend(pool, q, cu, lens, table, with_lse=True), *B.gather(pool, slots, torch.bfloat16)]
+
+    jobs = [job(), job()]
+    want = [[t.clone() for t in work(*j) + [j[0].k, j[0].v, j[0].k_scale, j[0].v_scale]] for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    got = [[], []]
+    for _ in range(6):
+        for s, (st, j) in enumerate(zip(streams, jobs)):
+            with torch.cuda.stream(st):
+                got[s].append(work(*j))
+    torch.cuda.synchronize()
+    for w, g, j in zip(want, got, jobs):
+        for x in g:
+            assert all(torch.equal(a, b) for a, b in zip(w, x))
+        assert all(torch.equal(a, b) for a, b in zip(w[4:], (j[0].k, j[0].v, j[0].k_scale, j[0].v_scale)))
 
 
 @pytest.mark.gpu
