@@ -981,13 +981,18 @@ constexpr int NARROW_ROWS = 256;
 constexpr int NARROW_CHUNK = 8;         // fewest 32-token tiles worth a part
 constexpr int WIDE_CHUNK = 16;
 
-// Parts of all kv heads that a read is divided into.  Narrow: as many as workgroups fit the chip at once (registers), which a larger
-// number only adds starts and parts to merge to (64 ragged requests of 128 dims: 512 parts 100 us, 1024 101, 2048 104; of 32 dims 1536
-// parts 33, 512 39).  Wide: the same at 128 dims (512 rows over 64 k tokens: 512 parts 674 us, 2048 748); smaller dims have shorter
-// units, which even out what a causal mask makes uneven (4 x 2000 causal rows of 64 dims: 2048 parts 165, 1024 180, 512 187; 4 x 1674
-// rows of 32 dims over 1.7 to 8.4 k tokens: 1536 parts 135, 2048 144, 1024 144, 512 163).
-int narrow_units(int dim) { return dim == 128 ? 512 : dim == 64 ? 1024 : 1536; }
-int wide_units(int dim) { return dim == 128 ? 512 : dim == 64 ? 2048 : 1536; }
+// Parts of all kv heads that a read is divided into: as many as there are workgroups on the chip at once (registers: two on each of 256
+// CUs at 128 dims, four of the wide kernel below; more parts add starts and more to merge, fewer leave CUs idle).  With 512 / 1024 /
+// 1536 / 2048 parts, us:
+//   wide, 8 x 32:    2 x 1000 fp32 rows over 5 k tokens 55 / 53 / 59 / 61, 4 x 1674 over 1.7 to 8.4 k 144 / 131 / 123 / 129,
+//                    6 x 500 causal rows of 4 x 2 heads over 3.5 k 53 / 50 / 52 / 52, 1 x 3600 over 18 k 220 / 218 / 217 / 224
+//   wide, 64 dims:   2 x 400 causal rows of 4 heads in one over 30 k 78 / 67 / 75 / 77, 3 x 2400 fp32 rows x 8 over 2.4 to 9.6 k
+//                    221 / 232 / 236 / 233
+//   narrow, 8 x 32:  64 rows over 16 to 33 k 37 / 35 / 35 / 34, 4 x 100 fp32 rows over 8 k 30 / 30 / 35 / 36
+// and with 256 / 512 / 1024 / 2048 parts at 128 dims:
+//   wide:            3 x 2400 fp32 rows x 8 over 2.4 to 9.6 k 581 / 505 / 521 / 537, 16 x 300 fp16 over 1 k 61 / 74 / 75 / 76
+//   narrow:          64 rows x 8 over 16 to 33 k 123 / 104 / 102 / 103, 4 x 100 fp32 rows over 8 k 52 / 53 / 60 / 72
+int parts_of(int dim) { return dim == 128 ? 512 : 1024; }
 
 struct Launch {
   Split sp;
@@ -1029,11 +1034,11 @@ Plan make_plan(const rmem_bank8_attn_args* a) {
   const long most = (long)a->max_rows * (a->heads_q / a->bank.heads);
   const int all = 0x7fffffff;
   Plan p = {};
-  if (most <= NARROW_ROWS) p.narrow = make_launch(a, most <= ROWS16 ? 16 : 32, narrow_units(a->bank.dim), NARROW_CHUNK, 0, all);
+  if (most <= NARROW_ROWS) p.narrow = make_launch(a, most <= ROWS16 ? 16 : 32, parts_of(a->bank.dim), NARROW_CHUNK, 0, all);
   else {
     // one request: the wide kernel alone; several: the short ones among them in a launch of their own
-    p.wide = make_launch(a, WROWS, wide_units(a->bank.dim), WIDE_CHUNK, a->reqs == 1 ? 0 : NARROW_ROWS + 1, all);
-    if (a->reqs > 1) p.narrow = make_launch(a, 32, narrow_units(a->bank.dim), NARROW_CHUNK, 0, NARROW_ROWS);
+    p.wide = make_launch(a, WROWS, parts_of(a->bank.dim), WIDE_CHUNK, a->reqs == 1 ? 0 : NARROW_ROWS + 1, all);
+    if (a->reqs > 1) p.narrow = make_launch(a, 32, parts_of(a->bank.dim), NARROW_CHUNK, 0, NARROW_ROWS);
   }
   return p;
 }
