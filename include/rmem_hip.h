@@ -539,8 +539,9 @@ int rmem_bank8_gather(const rmem_bank8_gather_args *a, void *stream);
  * rmem_bank8_plan did not grant are not in the bank, while its lens still counts what it had before: pass 0 for it.)
  * heads_q = a multiple of bank.heads: query head h reads head h / (heads_q / bank.heads).  q, out of `type` with strides in
  * elements and dim contiguous; lse [rows][heads_q] fp32 or NULL.  scale > 0.  max_rows: the largest number of rows of a request,
- * as far as known (it selects kernels; any value is safe).  Scores, weights and sums are fp32; q counts with 22 bits, values of
- * fp32 calls with 22-bit weights, of 16-bit calls with 11-bit weights.  Value scales below 2^-88 are read as 2^-88.
+ * as far as known (it selects kernels; any value is safe).  Scores, weights and sums are fp32.  16-bit q is exact (bf16 elements
+ * below 2^-31 of their row's largest: within 2^-39 of that), fp32 q within 2^-22 of the element or 2^-39 of its row's largest; values
+ * are multiplied by weights of 22 bits in fp32 calls, of 11 bits in 16-bit calls.  Value scales below 2^-88 are read as 2^-88.
  * (A request's value scales may differ by a factor of 2^100: beyond it the weights of the pages with the small ones would vanish.)
  * Refused: launches of 2^24 workgroups or more.  With G = heads_q / bank.heads a launch has, for each of bank.heads, rows * G / T of
  * them, min(reqs, rows) for tiles that are not full, and up to 2048 in all (at least one for each head) for what is divided; T = 16

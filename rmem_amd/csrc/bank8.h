@@ -1,5 +1,5 @@
-// bank8.h -- the paged 8-bit bank: storage, code conversions and the division of a read into units, shared by
-// bank8.hip (plan, append, gather) and bank8_attn.hip (the read).
+// bank8.h -- the paged 8-bit bank: storage, code conversions and argument checks, shared by bank8.hip (plan, append, gather) and
+// bank8_attn.hip (the read).
 //
 // A page holds `page` tokens of every head, one byte per element, laid out for the read's MFMA operands:
 //   keys    [page][head][dim/16][token][16]             a lane's 16 bytes = 16 dims of one token (A operand of S^T = K . Q^T)

@@ -285,8 +285,8 @@ __device__ __forceinline__ const T* element(const T* src, long ldr, int r, int a
 // them) leaves too few workgroups to hide the chain slots -> rows -> maximum -> codes.  Keys: a thread takes 16 dims of a token,
 // eight threads a token of 128 dims (256 bytes in, 128-byte pieces out).  Values: a thread takes 16 tokens (half a 32-token tile)
 // of two dims, so that a wave reads whole rows and each thread writes the two chunks that hold its tokens.
-// 25.6 k fp16 rows of 8 x 128 to e4m3: 48 us for 157 MB, 3.3 TB/s -- what is left is that chain, at 20 waves per CU (16: 50 us; 32 spill);
-// 64 single tokens 5.4 us.
+// 25.6 k fp16 rows of 8 x 128 to e4m3: 48 us for 157 MB, 3.3 TB/s -- what is left is that chain, at 20 waves per CU (16: 50 us; 32
+// spill, and at 20 the form for fp32 rows that are not 16-byte aligned, by two or three registers); 64 single tokens 5.4 to 5.9 us.
 template <class T, int CODE, int D, bool FAST, int NT>
 __global__ __launch_bounds__(NT, 5) void append_kernel(rmem_bank8_append_args a, const PageMark* marks, int ps, int window) {
   __shared__ float s_max[NT / 64];

@@ -7,8 +7,10 @@
 // Codes become fp16 exactly (8 bits fit into 11), so the key scale is applied to the scores, once per element beside the softmax
 // scale, and the value scale rides in the exponent: w = 2^(y - m), y = scale log2e ks s + log2 vs, O = sum w code, and the
 // denominator takes each tile's sum of weights times 1 / vs.  No dequantised value exists anywhere.
-// Queries enter as fp16 times a power of two per row that puts the row's largest element at 2^14: fp16 and bf16 rows are exact
-// down to 2^-38 of that element; fp32 rows keep 22 bits in two planes (NS = 2: two products against the same codes).
+// Queries enter as fp16.  fp16 rows as they are; bf16 and fp32 rows times a power of two that puts the row's largest element between
+// 2^14 and 2^15, where fp16's smallest step, 2^-24, is 2^-38 of 2^14: bf16 elements (8 bits) are exact down to 2^-31 of the largest
+// and below that off by at most half a step, 2^-39 of it; fp32 elements go into two planes (NS = 2: two products against the same
+// codes) and are off by at most 2^-22 of themselves or those 2^-39 of the row's largest, whichever is more.
 // Weights are 2^10 times their usual size (2^10 at the row's reference, not 1), which leaves 24 instead of 14 binades of normal
 // fp16 numbers below it; fp32 calls keep them in two planes.  Sums are fp32, of the unrounded weights.
 #include "bank8.h"
@@ -89,7 +91,7 @@ __device__ __forceinline__ int chunk_of(const Req& x, const Split& sp) {
 
 // With more requests than lanes the division is computed once, by a launch of its own (index_kernel), and looked up: what lies in
 // front of each request, and last the totals.  (Requests of one row and up to 1000 tokens, 64 at a time scanned by every workgroup:
-// 1000 of them 280 us, looked up 175 us; 200 of them 100 and 98.)
+// 1000 of them 280 us, looked up 175 us; 200 of up to 4000 tokens 100 and 98.)
 struct Before {
   int units, slots, ords, chunk;
 };
@@ -541,7 +543,9 @@ __device__ __forceinline__ void write_part(const Parts& w, const Acc<R, D>& c, c
 // Four waves share a unit of R rows: wave w takes token tiles w, w + 4, ..., straight from memory into operand registers, the
 // next tile's loads in flight behind the present one's arithmetic; the four partial results are joined through LDS.
 // Page ids and scales of a wave's next 64 tiles sit one per lane.  Bound by the bytes: one row of 64 heads over 250 k tokens of 8 x 128,
-// 512 MB, 90 us, 5.7 TB/s; 64 ragged rows of 32 heads, 451 MB, 88 us, 5.1 TB/s.
+// 512 MB, 92 us, 5.6 TB/s; 64 ragged rows of 32 heads, 451 MB, 91 us, 5.0 TB/s.  With 32 rows per tile the vector instructions bound
+// it, since each wave decodes what it multiplies: 64 requests of 16 tokens and 4 x 8 heads over 4 k tokens 110 us, 610 TFLOP/s,
+// vector pipe 66 % busy, matrix pipe 28 %.
 template <int R, int D>
 struct Raw;                               // a lane's codes of a tile
 template <int D>
@@ -735,8 +739,11 @@ __global__ __launch_bounds__(256, 2) void attn_narrow(rmem_bank8_attn_args a, Pa
 // Decoding ahead of LDS costs a wave a quarter of the conversions and doubles the LDS bytes: at 128 dims a wave reads 16 KB per 32
 // tokens, 512 clocks for four waves at 128 B per clock, as long as their matrix instructions; decoding behind it would put 128
 // conversions per 32 tokens beside every wave's softmax arithmetic, which is the longer pipe.
-// 512 rows of 32 heads over 64 k tokens of 128 dims: 680 us, 810 TFLOP/s, matrix pipe busy 37 % of the time, vector pipe 60 %.  Computing a
+// 512 rows of 32 heads over 64 k tokens of 128 dims: 678 us, 814 TFLOP/s, matrix pipe busy 40 % of the time, vector pipe 56 %.  Computing a
 // stage's scores beside the former's weights needs 230 registers, and loses more by the wave that then does not fit (790 us).
+// fp32 rows, two planes of queries and weights: 4 x 1674 rows x 8 over 1.7 to 8.4 k tokens of 64 dims 173 us, matrix pipe 35 %, vector
+// pipe 55 %; of 128 dims one wave per SIMD (219 + 96 registers), which hides little: 450 us, 24 % and 29 %; 2 x 2048 causal rows of 32
+// heads over 10 k tokens 1.43 ms, 35 % and 38 %, against 702 us for bf16 rows.
 constexpr int WROWS = 128;
 
 template <int D, int CODE, int NS>
@@ -975,8 +982,10 @@ __global__ __launch_bounds__(256) void attn_merge_both(rmem_bank8_attn_args a, P
 
 // -------------------------------------------------------------------------------------------------------------------- host
 constexpr int ROWS16 = 16;              // requests of at most this many rows per kv head take tiles of 16 rows
-// Up to this many the narrow kernel, beyond the wide one.  4 requests of 256 rows over 16 k tokens of 128 dims: narrow 61 us, wide 72;
-// of 256 single-head rows over 8 k tokens of 64 dims: 44 and 67; 512 causal rows over 64 k tokens: the wide kernel, 820 TFLOP/s.
+// Up to this many the narrow kernel, beyond the wide one.  Narrow and wide, with their merges, us: 4 requests of 32 tokens and 4 x 8
+// heads (256 rows per kv head) over 16 k tokens of 128 dims 59, 70; 4 of 256 tokens and 8 heads over 8 k of 64 dims 41, 56; 20 of 130
+// fp32 tokens and 8 heads over 2 k of 32 dims 40, 49; one of 60 tokens and 8 x 4 heads over 20 k of 128 dims 41, 50; 64 of 16 tokens and
+// 4 x 8 heads over 4 k of 128 dims 115, 114.
 constexpr int NARROW_ROWS = 256;
 constexpr int NARROW_CHUNK = 8;         // fewest 32-token tiles worth a part
 constexpr int WIDE_CHUNK = 16;
